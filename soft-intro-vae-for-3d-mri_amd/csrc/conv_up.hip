@@ -371,18 +371,9 @@ __global__ __launch_bounds__(256, 2) void k2_up_fwd_prod(const float* __restrict
     for (int i = 0; i < PD; ++i) SIV_PIN(bring[i]);
 #undef SIV_PIN
 
-    // four-channel differences as two packed two-channel subtractions (vector instructions take matrix-pipe
-    // time on a SIMD that runs fp32 matrix instructions, so their count matters)
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     struct f32x4 { f32x2 lo, hi; };
-    // (spelled as the instruction: the compiler splits a packed subtraction whose halves feed different
-    // matrix instructions into two scalar ones)
-    auto pk_sub = [](f32x2 a, f32x2 c) {
-        f32x2 r;
-        asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(r) : "v"(a), "v"(c));
-        return r;
-    };
-    auto sub4 = [&](f32x4 a, f32x4 c) { return f32x4{pk_sub(a.lo, c.lo), pk_sub(a.hi, c.hi)}; };
+    auto sub4 = [&](f32x4 a, f32x4 c) { return f32x4{a.lo - c.lo, a.hi - c.hi}; };
     for (int cc = 0; cc < nchunk; ++cc) {
         __syncthreads();
 #pragma unroll

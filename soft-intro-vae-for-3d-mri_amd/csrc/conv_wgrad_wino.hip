@@ -57,8 +57,8 @@ struct GwGeom {
 // The factors 1/2 of G (positions 1 and 2 along either axis) are left out of the dy transform and applied
 // to the finished sums (exact: powers of two).  A sample is read through a buffer descriptor whose per-lane
 // offset carries voxel AND plane, so a voxel or a whole plane outside the volume reads zeros: no masks, no
-// 64-bit address arithmetic, and the transforms are packed two-channel operations -- every vector
-// instruction a wave issues here takes time on the matrix pipe.
+// 64-bit address arithmetic, and the transforms take two channels at a time.  Every vector instruction
+// a wave issues here takes time on the matrix pipe.
 template <bool ISV>
 __device__ __forceinline__ void gw_run(const float* __restrict__ src, const int chan, const int Cs,
                                        f32x16 (&acc)[3][2], float* lds, const int ph, const int set,

@@ -46,7 +46,7 @@ __device__ unsigned long long w2_stamps[2048 * 8 * 32];
 #endif
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));    // two channels per lane: one packed add per pair
+typedef float f32x2 __attribute__((ext_vector_type(2)));    // two channels per lane
 constexpr unsigned W2_OUTSIDE = 0x80000000u;      // beyond any sample (the launcher keeps samples below 2 GiB)
 
 struct W2Cfg {
