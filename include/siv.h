@@ -36,6 +36,11 @@ extern "C" {
 #define SIV_EWORKSPACE (-2)  /* workspace too small */
 #define SIV_EHIP (-3)        /* a HIP runtime call or kernel launch failed */
 
+/* Element types of the operators that take more than fp32 (siv_layer_norm_*, siv_add_layer_norm_*, siv_dropout_*) */
+#define SIV_F32 0
+#define SIV_BF16 1
+#define SIV_F16 2
+
 typedef void* siv_stream_t;  /* hipStream_t */
 
 const char* siv_last_error(void);
@@ -407,6 +412,55 @@ int siv_act_dropout_fwd(const float* x, const uint8_t* keep, float p, float slop
                         float* out, long n, siv_stream_t stream);
 int siv_act_dropout_bwd(const float* dout, const float* x, const uint8_t* keep, float p,
                         float slope, float* dx, long n, siv_stream_t stream);
+
+/* ---- layer normalisation -----------------------------------------------------------------------
+ * No reference counterpart: the reference normalises with nn.BatchNorm3d only (models/models.py:18,22,56,60,93,119),
+ * whose statistics are those of a single sample at batch 1.  A row is what one normalisation spans: the C channels of
+ * a voxel (rows = N*D*H*W of an NDHWC tensor) or the last axis of any row-major tensor.
+ *   mean = sum x / C, var = sum (x - mean)^2 / C, h = (x - mean) / sqrt(var + eps), y = h * weight + bias
+ *   g = dy * weight, dx = (g - sum g / C - h * sum(g h) / C) / sqrt(var + eps)
+ *   dweight = sum_rows dy * h, dbias = sum_rows dy
+ *  - `type` (SIV_F32 / SIV_BF16 / SIV_F16) is the type of every activation tensor of the call; statistics, sums and
+ *    all arithmetic are fp32, results are rounded to nearest even once.  weight / bias (and their gradients) are
+ *    [C] of `wtype`: SIV_F32 or `type`; either may be NULL (factor 1 / offset 0).
+ *  - x and dy are rows of C consecutive elements, ldx / lddy elements apart (>= C); y and dx are dense.  Any
+ *    alignment of the element type is accepted.  x must not overlap y / dx.
+ *  - forward keeps nothing for backward: the statistics are formed again from x.
+ *  - dx, dweight, dbias may be NULL; accumulate != 0 adds into dweight / dbias.  Their sums have a fixed order.
+ *  - ws: siv_layer_norm_workspace writes the bytes the forward (backward = 0) or backward (1) call of that size
+ *    needs to *bytes, a HOST address; 0 = ws may be NULL. */
+int siv_layer_norm_workspace(long rows, long C, int type, int backward, size_t* bytes);
+int siv_layer_norm_fwd(const void* x, long ldx, const void* weight, const void* bias, int wtype, float eps,
+                       void* y, int type, long rows, long C, void* ws, size_t ws_bytes, siv_stream_t stream);
+int siv_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, const void* weight, int wtype,
+                       float eps, void* dx, void* dweight, void* dbias, int accumulate, int type, long rows,
+                       long C, void* ws, size_t ws_bytes, siv_stream_t stream);
+/* The closing step of a residual branch in one pass: s = residual + dropout(x), held in `type`, and
+ * y = layer_norm(s) of what is held.  All tensors are dense [rows][C].  Dropout as in siv_dropout_fwd (element i of
+ * x is drawn at index i); p == 0 with keep == NULL adds x itself.
+ * _bwd: dy and ds (NULL = zero) are the gradients of y and s; dresidual = ds + the norm's input gradient,
+ * dx = dropout's backward of it; any of the four results may be NULL.  Workspace as for siv_layer_norm_*. */
+int siv_add_layer_norm_fwd(const void* x, const void* residual, const uint8_t* keep, uint64_t seed,
+                           uint64_t stream_id, const uint64_t* epoch, float p, const void* weight,
+                           const void* bias, int wtype, float eps, void* s, void* y, int type, long rows,
+                           long C, void* ws, size_t ws_bytes, siv_stream_t stream);
+int siv_add_layer_norm_bwd(const void* dy, const void* ds, const void* s, const uint8_t* keep, uint64_t seed,
+                           uint64_t stream_id, const uint64_t* epoch, float p, const void* weight, int wtype,
+                           float eps, void* dx, void* dresidual, void* dweight, void* dbias, int accumulate,
+                           int type, long rows, long C, void* ws, size_t ws_bytes, siv_stream_t stream);
+/* Dropout whose mask is never stored: out[i] = [residual[i] +] (kept(i) ? act(x[i]) / (1 - p) : 0) with
+ * act = LeakyReLU(slope), slope 1 = identity: nn.ReLU + nn.Dropout(0.35) of models/models.py:139-140 and any other
+ * nn.Dropout.  kept(i): keep[i] != 0 where a mask tensor is given; else, for p > 0, drawn by the kernel -- component
+ * i % 4 of Philox(i / 4, stream_id [+ *epoch * 2^20], seed), the bits siv_dropout_keep(_at) writes for the same key;
+ * else always.  A dropped element contributes 0 whatever x holds there (NaN and infinities included).
+ * _bwd draws again: dx[i] = (kept(i) ? dout[i] / (1 - p) : 0) * act'(x[i]); x may be NULL where slope == 1.  The
+ * gradient of the residual is dout itself.  n elements of `type` in memory order; out / dx may alias nothing. */
+int siv_dropout_fwd(const void* x, const void* residual, const uint8_t* keep, uint64_t seed, uint64_t stream_id,
+                    const uint64_t* epoch, float p, float slope, void* out, int type, long n,
+                    siv_stream_t stream);
+int siv_dropout_bwd(const void* dout, const void* x, const uint8_t* keep, uint64_t seed, uint64_t stream_id,
+                    const uint64_t* epoch, float p, float slope, void* dx, int type, long n,
+                    siv_stream_t stream);
 
 /* ---- latent sampling and losses -------------------------------------------------
  * z = mu + eps*exp(0.5*logvar): SoftIntroVAE.reparameterize, models/models.py:263-271.

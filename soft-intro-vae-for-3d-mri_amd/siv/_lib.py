@@ -74,6 +74,14 @@ SIGNATURES = {
                             _i, _i, _i, _i, _i, _i, _f, _sz, _f],
     "siv_act_dropout_fwd": [_f, _f, _fl, _fl, _f, _l, _f],
     "siv_act_dropout_bwd": [_f, _f, _f, _fl, _fl, _f, _l, _f],
+    "siv_dropout_fwd": [_f, _f, _f, _u64, _u64, _f, _fl, _fl, _f, _i, _l, _f],
+    "siv_dropout_bwd": [_f, _f, _f, _u64, _u64, _f, _fl, _fl, _f, _i, _l, _f],
+    "siv_layer_norm_workspace": [_l, _l, _i, _i, _f],
+    "siv_layer_norm_fwd": [_f, _l, _f, _f, _i, _fl, _f, _i, _l, _l, _f, _sz, _f],
+    "siv_layer_norm_bwd": [_f, _l, _f, _l, _f, _i, _fl, _f, _f, _f, _i, _i, _l, _l, _f, _sz, _f],
+    "siv_add_layer_norm_fwd": [_f, _f, _f, _u64, _u64, _f, _fl, _f, _f, _i, _fl, _f, _f, _i, _l, _l, _f, _sz, _f],
+    "siv_add_layer_norm_bwd": [_f, _f, _f, _f, _u64, _u64, _f, _fl, _f, _i, _fl, _f, _f, _f, _f, _i, _i, _l, _l, _f, _sz,
+                               _f],
     "siv_reparam_fwd": [_f, _f, _f, _fl, _f, _l, _f],
     "siv_reparam_bwd": [_f, _f, _f, _fl, _f, _f, _l, _f],
     "siv_kl_fwd": [_f, _f, _f, _i, _l, _f],

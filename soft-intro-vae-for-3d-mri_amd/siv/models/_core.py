@@ -349,7 +349,7 @@ class ResNetDecoder(nn.Module):
             h = ops.bn_act_conv_to1(y, last.block[5], v.slope, conv, self.training, stats)
         else:
             h = ops.conv3d_k3(h, conv.weight, conv.bias)
-        keep = _keep(h.shape, v.p_dec_out, self.training, h.device)
+        keep = _keep(h.shape, v.p_dec_out, self.training, h.device, stored=not ops.draws_masks())
         return ops.act_dropout(h, 0.0, keep=keep, p=v.p_dec_out)   # nn.ReLU then nn.Dropout
 
 

@@ -9,6 +9,7 @@ from typing import Optional
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import activations
 from .backend import get_backend
@@ -604,8 +605,129 @@ class _ActDropout(Function):
 
 
 def act_dropout(x, slope: float, keep=None, p: float = 0.0):
-    """LeakyReLU(slope) (slope 0 = ReLU) followed by dropout with an explicit keep mask."""
+    """LeakyReLU(slope) (slope 0 = ReLU) followed by dropout.  ``keep`` is a uint8 mask tensor, or a
+    ``rng.PhiloxKeep`` key (``draws_masks()``): the kernels then draw the mask themselves, forward and backward, and no
+    mask tensor exists."""
+    if keep is not None and not torch.is_tensor(keep):
+        return _Dropout.apply(x, None, keep, p, slope)
     return _ActDropout.apply(x, keep, p, slope)
+
+
+def draws_masks() -> bool:
+    """True where ``dropout`` / ``act_dropout`` / ``add_layer_norm`` take a ``rng.PhiloxKeep`` key as ``keep``."""
+    return getattr(get_backend(), "draws_masks", False)
+
+
+def _mask_of(keep):
+    """(mask tensor or None, key or None): the two places a dropout mask can come from."""
+    return (keep, None) if torch.is_tensor(keep) else (None, keep)
+
+
+class _Dropout(Function):
+    @staticmethod
+    def forward(ctx, x, residual, keep, p, slope):
+        mask, ctx.key = _mask_of(keep)
+        ctx.save_for_backward(x if slope != 1.0 else None, mask)
+        ctx.cfg = (p, slope)
+        return get_backend().dropout_fwd(x, keep, p, slope, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        dx = None
+        if ctx.needs_input_grad[0]:
+            x, mask = ctx.saved_tensors
+            dx = get_backend().dropout_bwd(dout, x, mask if ctx.key is None else ctx.key, *ctx.cfg)
+        return dx, (dout if ctx.needs_input_grad[1] else None), None, None, None
+
+
+def dropout(x, keep, p: float, residual=None):
+    """nn.Dropout(p) with its mask given: ``x * keep / (1 - p)``, onto ``residual`` where one is given, in one pass.
+    ``keep``: a ``rng.PhiloxKeep`` key (``rng.get_rng().keep_mask_key(x.shape, p, x.device)``), whose mask is drawn by
+    the kernels, forward and backward, and never stored; a uint8 mask tensor; or None (nothing dropped).  A dropped
+    element contributes 0 whatever ``x`` holds there.  float32, bfloat16 or float16, any shape."""
+    return _Dropout.apply(x, residual, keep, p, 1.0)
+
+
+class _LayerNorm(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y = get_backend().layer_norm_fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight)
+        ctx.cfg = (eps, _param_dtype(weight, bias))
+        ctx.bufs = (_grad_buf(weight), _grad_buf(bias))
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        eps, pdtype = ctx.cfg
+        wb = _affine_bufs(ctx.bufs, need_w, need_b)
+        dx, dw, db = get_backend().layer_norm_bwd(dy, x, weight, eps, pdtype, need_x, need_w, need_b, *wb)
+        return (dx, dw, db, None) if wb == (None, None) else (dx, None, None, None)
+
+
+def _param_dtype(weight, bias):
+    for w in (weight, bias):
+        if w is not None:
+            return w.dtype
+    return torch.float32
+
+
+def _affine_bufs(bufs, need_w, need_b):
+    """The flat-buffer views both parameter gradients are added into, or (None, None) where one of them has none."""
+    w_buf, b_buf = bufs
+    if (need_w and w_buf is None) or (need_b and b_buf is None):
+        return None, None
+    return (w_buf if need_w else None), (b_buf if need_b else None)
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
+    """nn.LayerNorm over the channels of every voxel (5-D tensors, NCDHW) or over the last axis (any other rank):
+    ``(x - mean) / sqrt(var + eps) * weight + bias`` with the row's own mean and biased variance -- no batch, no running
+    statistics.  float32, bfloat16 or float16; ``weight`` / ``bias`` float32 or of x's type, or None.  Rows may be slices
+    of wider rows.  Statistics are fp32 and formed again by the backward pass; only ``x`` is kept."""
+    return _LayerNorm.apply(x, weight, bias, eps)
+
+
+class _AddLayerNorm(Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, keep, p):
+        y, s = get_backend().add_layer_norm_fwd(x, residual, keep, p, weight, bias, eps)
+        mask, ctx.key = _mask_of(keep)
+        ctx.save_for_backward(s, weight, mask)
+        ctx.cfg = (eps, p, _param_dtype(weight, bias))
+        ctx.bufs = (_grad_buf(weight), _grad_buf(bias))
+        ctx.set_materialize_grads(False)
+        return y, s
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds):
+        s, weight, mask = ctx.saved_tensors
+        eps, p, pdtype = ctx.cfg
+        keep = mask if ctx.key is None else ctx.key
+        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
+        if dy is None:              # only the sum went on: the norm takes no part
+            if ds is None:
+                return (None,) * 7
+            dx = get_backend().dropout_bwd(ds, None, keep, p) if need_x else None
+            return dx, (ds if need_r else None), None, None, None, None, None
+        wb = _affine_bufs(ctx.bufs, need_w, need_b)
+        dx, dres, dw, db = get_backend().add_layer_norm_bwd(dy, ds, s, keep, p, weight, eps, pdtype, need_x, need_r,
+                                                            need_w, need_b, *wb)
+        if wb != (None, None):
+            dw = db = None
+        return dx, dres, dw, db, None, None, None
+
+
+def add_layer_norm(x, residual, weight=None, bias=None, eps: float = 1e-5, keep=None, p: float = 0.0):
+    """The closing step of a residual branch in one pass: ``s = residual + dropout(x)`` and ``y = layer_norm(s)``;
+    returns ``(y, s)``.  ``keep`` / ``p`` as in ``dropout``, rows and parameters as in ``layer_norm``; ``s`` is held in
+    the tensors' type and it is what is normalised."""
+    return _AddLayerNorm.apply(x, residual, weight, bias, eps, keep, p)
 
 
 class _Reparam(Function):
