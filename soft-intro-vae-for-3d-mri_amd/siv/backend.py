@@ -764,14 +764,15 @@ class HipBackend:
         return (None, keep.seed & m, keep.stream_id & m, _p(e), p), e
 
     def _launch(self, what, x, *args):
-        """Call the entry point ``what`` on the current stream of x's device, with that device current."""
-        st = torch.cuda.current_stream(x.device).cuda_stream
+        """Call the entry point ``what`` on the current stream of x's device, with that device current.  (The raw
+        accessors: torch.cuda.current_stream / current_device cost microseconds on autograd's threads.)"""
+        dev = x.get_device()
         fn = getattr(self.lib, what)
-        if x.device.index == torch.cuda.current_device():
-            rc = fn(*args, st)
+        if torch._C._cuda_getDevice() == dev:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
         else:
-            with torch.cuda.device(x.device):
-                rc = fn(*args, st)
+            with torch.cuda.device(dev):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
         if rc != 0:
             _lib.check(rc, what)
 
