@@ -1,48 +1,75 @@
 // Dropout whose mask is never stored (fp32, bf16, fp16): out = [residual +] keep * act(x) / (1 - p).
+// Element i of a call is component i % 4 of Philox(i / 4, stream id, seed): forward and backward draw it again instead
+// of writing and reading a mask.
 #include "elem_types.h"
 
 namespace siv {
 
-// One thread per quad of elements: one Philox call is four of them.
-template <typename T>
-__global__ __launch_bounds__(256) void dropout_fwd_k(const T* __restrict__ x, const T* __restrict__ res, Drop d,
-                                                     float slope, T* __restrict__ out, long n) {
+// 256 threads take a tile of 256 packs of 16 bytes at a time, one each.  The tile starts at a multiple of 2^8 Philox
+// calls, so the upper counter word, like stream id and key, is the same for the whole block: a tenth of the products
+// of the generator's first two rounds stay on the scalar unit.
+template <typename T, bool AL, bool RES, bool BWD>
+__global__ __launch_bounds__(256) void dropout_k(const T* __restrict__ in, const T* __restrict__ other, Drop d,
+                                                 float slope, T* __restrict__ out, long n) {
+    constexpr int N = Pack<T>::N;
     const uint64_t sid = drop_sid(d);
-    const long quads = (n + 3) / 4;
-    for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < quads; q += (long)gridDim.x * 256) {
-        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
-        if (d.mode == 1) {
-            const u4 r = philox4x32_10((uint64_t)q, sid, d.seed);
-            w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+    const long tiles = (n + 256 * N - 1) / (256 * N);
+    for (long t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const long i = t * (256 * N) + threadIdx.x * N, have = n - i;
+        const bool whole = have >= N;
+        const Pack<T> p = whole ? load_pack<AL>(in + i, N) : load_pack<false>(in + i, have);
+        Pack<T> q;
+        if (other) q = whole ? load_pack<AL>(other + i, N) : load_pack<false>(other + i, have);
+        float v[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = BWD ? (float)p.e[j] : leaky((float)p.e[j], slope);
+        if (d.mode) {
+            uint32_t w[N];
+            if (d.mode == 1) {
+                const uint64_t q0 = (uint64_t)t * (256 * N / 4);
+#pragma unroll
+                for (int k = 0; k < N / 4; ++k) {
+                    const u4 r = philox4x32_10((q0 & ~0xffffffffull) | ((uint32_t)q0 + threadIdx.x * (N / 4) + k), sid, d.seed);
+                    w[4 * k] = r.x;
+                    w[4 * k + 1] = r.y;
+                    w[4 * k + 2] = r.z;
+                    w[4 * k + 3] = r.w;
+                }
+            } else {
+                stored_words<N>(d, i, have, w);
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = w[j] >= d.least ? v[j] * d.scale : 0.f;
         }
-        for (int j = 0; j < 4; ++j) {
-            const long i = q * 4 + j;
-            if (i >= n) break;
-            float v = leaky((float)x[i], slope);
-            if (d.mode) v = (d.mode == 1 ? (w[j] >> 8) >= d.thresh : d.keep[i] != 0) ? v * d.scale : 0.f;
-            out[i] = (T)(res ? (float)res[i] + v : v);
+        Pack<T> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (BWD && other) v[j] *= leaky_grad((float)q.e[j], slope);
+            if (RES) v[j] = (float)q.e[j] + v[j];
+            o.e[j] = (T)v[j];
         }
+        if (whole) store_pack<AL>(out + i, N, o);
+        else store_pack<false>(out + i, have, o);
     }
 }
-template <typename T>
-__global__ __launch_bounds__(256) void dropout_bwd_k(const T* __restrict__ dout, const T* __restrict__ x, Drop d,
-                                                     float slope, T* __restrict__ dx, long n) {
-    const uint64_t sid = drop_sid(d);
-    const long quads = (n + 3) / 4;
-    for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < quads; q += (long)gridDim.x * 256) {
-        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
-        if (d.mode == 1) {
-            const u4 r = philox4x32_10((uint64_t)q, sid, d.seed);
-            w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
-        }
-        for (int j = 0; j < 4; ++j) {
-            const long i = q * 4 + j;
-            if (i >= n) break;
-            float g = (float)dout[i];
-            if (d.mode) g = (d.mode == 1 ? (w[j] >> 8) >= d.thresh : d.keep[i] != 0) ? g * d.scale : 0.f;
-            dx[i] = (T)(x ? g * leaky_grad((float)x[i], slope) : g);
-        }
-    }
+
+// in / other: x and the residual (forward), dout and x (backward)
+template <bool BWD>
+static int dropout(const char* what, const void* in, const void* other, const Drop& d, float slope, void* out, int type,
+                   long n, hipStream_t st) {
+    const bool al = aligned16(in) && aligned16(other) && aligned16(out);
+    return with_type(type, [&](auto* t) {
+        typedef typename std::remove_reference<decltype(*t)>::type T;
+        const long tiles = cdiv(n, 256 * Pack<T>::N);
+        const unsigned g = (unsigned)(tiles < 4096 ? tiles : 4096);
+        const T *a = (const T*)in, *b = (const T*)other;
+        if (al && (BWD || !b)) dropout_k<T, true, false, BWD><<<g, 256, 0, st>>>(a, b, d, slope, (T*)out, n);
+        else if (al) dropout_k<T, true, !BWD, BWD><<<g, 256, 0, st>>>(a, b, d, slope, (T*)out, n);
+        else if (BWD || !b) dropout_k<T, false, false, BWD><<<g, 256, 0, st>>>(a, b, d, slope, (T*)out, n);
+        else dropout_k<T, false, !BWD, BWD><<<g, 256, 0, st>>>(a, b, d, slope, (T*)out, n);
+        SIV_CHECK_LAUNCH(what);
+        return SIV_OK;
+    });
 }
 
 }  // namespace siv
@@ -58,15 +85,8 @@ extern "C" int siv_dropout_fwd(const void* x, const void* residual, const uint8_
                                int type, long n, siv_stream_t stream) {
     SIV_CHECK_ARG(x && out && n > 0, "dropout_fwd: bad argument");
     SIV_CHECK_DROP("dropout_fwd");
-    const Drop d = make_drop(keep, seed, stream_id, epoch, p);
-    return with_type(type, [&](auto* t) {
-        typedef typename std::remove_reference<decltype(*t)>::type T;
-        const long g = cdiv(cdiv(n, 4), 256);
-        dropout_fwd_k<T><<<(unsigned)(g > 4096 ? 4096 : g), 256, 0, (hipStream_t)stream>>>(
-            (const T*)x, (const T*)residual, d, slope, (T*)out, n);
-        SIV_CHECK_LAUNCH("dropout_fwd");
-        return SIV_OK;
-    });
+    return dropout<false>("dropout_fwd", x, residual, make_drop(keep, seed, stream_id, epoch, p), slope, out, type, n,
+                          (hipStream_t)stream);
 }
 extern "C" int siv_dropout_bwd(const void* dout, const void* x, const uint8_t* keep, uint64_t seed,
                                uint64_t stream_id, const uint64_t* epoch, float p, float slope, void* dx, int type,
@@ -74,13 +94,6 @@ extern "C" int siv_dropout_bwd(const void* dout, const void* x, const uint8_t* k
     SIV_CHECK_ARG(dout && dx && n > 0, "dropout_bwd: bad argument");
     SIV_CHECK_ARG(x || slope == 1.f, "dropout_bwd: the activation's backward needs x");
     SIV_CHECK_DROP("dropout_bwd");
-    const Drop d = make_drop(keep, seed, stream_id, epoch, p);
-    return with_type(type, [&](auto* t) {
-        typedef typename std::remove_reference<decltype(*t)>::type T;
-        const long g = cdiv(cdiv(n, 4), 256);
-        dropout_bwd_k<T><<<(unsigned)(g > 4096 ? 4096 : g), 256, 0, (hipStream_t)stream>>>(
-            (const T*)dout, slope == 1.f ? nullptr : (const T*)x, d, slope, (T*)dx, n);
-        SIV_CHECK_LAUNCH("dropout_bwd");
-        return SIV_OK;
-    });
+    return dropout<true>("dropout_bwd", dout, slope == 1.f ? nullptr : x, make_drop(keep, seed, stream_id, epoch, p),
+                         slope, dx, type, n, (hipStream_t)stream);
 }

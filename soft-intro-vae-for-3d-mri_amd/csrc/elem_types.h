@@ -65,50 +65,64 @@ struct Drop {
     const uint8_t* keep;              // stored mask, element order of the tensor
     uint64_t seed, sid;
     const unsigned long long* epoch;
-    uint32_t thresh;                  // an element is kept when the top 24 bits of its word are >= thresh
+    uint32_t least;                   // an element is kept when its word is >= least
     float scale;                      // 1 / (1 - p)
     int mode;                         // 0: keep everything, 1: draw, 2: read `keep`
 };
-// p in [0, 1): the smallest 24-bit integer t with t * 2^-24 >= p, so that the integer comparison is philox_keeps
+// p in [0, 1).  A drawn element is kept when the top 24 bits of its word, as a fraction, are >= p (philox_keeps), i.e.
+// when the word is >= ceil(p 2^24) 2^8, which is at most (2^24 - 1) 2^8 for p < 1.  A stored mask's words are 0 or ~0.
 static inline Drop make_drop(const uint8_t* keep, uint64_t seed, uint64_t sid, const uint64_t* epoch, float p) {
     Drop d;
     d.keep = keep;
     d.seed = seed;
     d.sid = sid;
     d.epoch = (const unsigned long long*)epoch;
-    const double t = (double)p * 16777216.0;
-    d.thresh = (uint32_t)t;
-    if ((double)d.thresh < t) ++d.thresh;
-    d.scale = 1.0f / (1.0f - p);
     d.mode = keep ? 2 : (p > 0.f ? 1 : 0);
+    const double t = (double)p * 16777216.0;
+    uint32_t k = (uint32_t)t;
+    if ((double)k < t) ++k;
+    d.least = d.mode == 1 ? k << 8 : 1;
+    d.scale = 1.0f / (1.0f - p);
     return d;
 }
 __device__ __forceinline__ uint64_t drop_sid(const Drop& d) {
     return (d.mode == 1 && d.epoch) ? d.sid + *d.epoch * SIV_EPOCH_STRIDE : d.sid;
 }
-// Bits 0 .. N-1: elements i .. i+N-1 are kept; of those, only the first `have` exist (others: unspecified).  QUAD: i is
-// a multiple of 4, so the N elements are whole Philox calls; otherwise one call more and a shift.
-template <int N, bool QUAD>
-__device__ __forceinline__ uint32_t drop_bits(const Drop& d, uint64_t sid, long i, long have) {
-    if (d.mode == 0) return ~0u;
-    uint32_t bits = 0;
-    if (d.mode == 2) {
+// Words of elements i .. i+N-1 of a stored mask, of which the first `have` exist.
+template <int N>
+__device__ __forceinline__ void stored_words(const Drop& d, uint64_t i, long have, uint32_t (&w)[N]) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < have) bits |= (uint32_t)(d.keep[i + j] != 0) << j;
-        return bits;
-    }
-    const uint64_t q = (uint64_t)i >> 2;
+    for (int j = 0; j < N; ++j) w[j] = (j < have && d.keep[i + j]) ? ~0u : 0u;
+}
+// The same drawn.  QUAD: i is a multiple of 4, so the N elements are whole Philox calls; otherwise one call more and a
+// shift by 0 to 3 words.
+template <int N, bool QUAD>
+__device__ __forceinline__ void drawn_words(const Drop& d, uint64_t sid, uint64_t i, uint32_t (&w)[N]) {
+    const uint64_t q = i >> 2;
     constexpr int CALLS = N / 4 + (QUAD ? 0 : 1);
+    uint32_t v[CALLS * 4];
 #pragma unroll
     for (int k = 0; k < CALLS; ++k) {
         const u4 r = philox4x32_10(q + k, sid, d.seed);
-        bits |= (uint32_t)((r.x >> 8) >= d.thresh) << (4 * k);
-        bits |= (uint32_t)((r.y >> 8) >= d.thresh) << (4 * k + 1);
-        bits |= (uint32_t)((r.z >> 8) >= d.thresh) << (4 * k + 2);
-        bits |= (uint32_t)((r.w >> 8) >= d.thresh) << (4 * k + 3);
+        v[4 * k] = r.x;
+        v[4 * k + 1] = r.y;
+        v[4 * k + 2] = r.z;
+        v[4 * k + 3] = r.w;
     }
-    return QUAD ? bits : bits >> ((uint32_t)i & 3);
+    if (!QUAD) {
+#pragma unroll
+        for (int j = 0; j + 1 < CALLS * 4; ++j) v[j] = (i & 1) ? v[j + 1] : v[j];
+#pragma unroll
+        for (int j = 0; j + 2 < CALLS * 4; ++j) v[j] = (i & 2) ? v[j + 2] : v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = v[j];
+}
+// modes 1 and 2
+template <int N, bool QUAD>
+__device__ __forceinline__ void drop_words(const Drop& d, uint64_t sid, uint64_t i, long have, uint32_t (&w)[N]) {
+    if (d.mode == 2) stored_words<N>(d, i, have, w);
+    else drawn_words<N, QUAD>(d, sid, i, w);
 }
 
 }  // namespace siv

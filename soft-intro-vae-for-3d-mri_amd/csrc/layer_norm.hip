@@ -106,13 +106,16 @@ template <typename T, bool AL>
 __device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res, const Drop& d, uint64_t sid, long i,
                                             long have) {
     constexpr int N = Pack<T>::N;
-    const uint32_t bits = drop_bits<N, AL>(d, sid, i, have);
     Pack<T> s;
+    if (d.mode == 0) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const float v = (float)x.e[j];
-        s.e[j] = (T)((float)res.e[j] + (d.mode ? ((bits >> j & 1) ? v * d.scale : 0.f) : v));
+        for (int j = 0; j < N; ++j) s.e[j] = (T)((float)res.e[j] + (float)x.e[j]);
+        return s;
     }
+    uint32_t w[N];
+    drop_words<N, AL>(d, sid, i, have, w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) s.e[j] = (T)((float)res.e[j] + (w[j] >= d.least ? (float)x.e[j] * d.scale : 0.f));
     return s;
 }
 
@@ -274,9 +277,10 @@ __global__ __launch_bounds__(256) void ln_bwd_k(NormArgs a, Drop d) {
             }
             if (a.dx) {
                 if (d.mode && hv > 0) {
-                    const uint32_t bits = drop_bits<N, AL>(d, sid, i, hv);
+                    uint32_t u[N];
+                    drop_words<N, AL>(d, sid, i, hv, u);
 #pragma unroll
-                    for (int j = 0; j < N; ++j) g[j] = (bits >> j & 1) ? g[j] * d.scale : 0.f;
+                    for (int j = 0; j < N; ++j) g[j] = u[j] >= d.least ? g[j] * d.scale : 0.f;
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j) p.e[j] = (T)g[j];
@@ -523,9 +527,10 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
             }
             if (a.dx) {
                 if (d.mode && hv > 0) {
-                    const uint32_t bits = drop_bits<N, AL>(d, sid, i, hv);
+                    uint32_t u[N];
+                    drop_words<N, AL>(d, sid, i, hv, u);
 #pragma unroll
-                    for (int j = 0; j < N; ++j) g[j] = (bits >> j & 1) ? g[j] * d.scale : 0.f;
+                    for (int j = 0; j < N; ++j) g[j] = u[j] >= d.least ? g[j] * d.scale : 0.f;
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j) o.e[j] = (T)g[j];

@@ -9,6 +9,7 @@ can substitute a checker when exercising the host logic on a machine without a G
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -31,6 +32,15 @@ def like(t: torch.Tensor) -> torch.Tensor:
 
 def empty_cl(shape, like: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
     return torch.empty(tuple(shape), device=like.device, dtype=dtype, memory_format=CL3D)
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_ws_bytes(rows: int, C: int, t: int, backward: int) -> int:
+    """What siv_layer_norm_workspace says (a function of the sizes alone)."""
+    n = ctypes.c_size_t()
+    _lib.check(_lib.load().siv_layer_norm_workspace(rows, C, t, backward, ctypes.addressof(n)),
+               "siv_layer_norm_workspace")
+    return n.value
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -671,34 +681,36 @@ class HipBackend:
         return dx
 
     # ---- layer normalisation, dropout without a stored mask (fp32, bf16, fp16) --------------------------
+    # A call on a small tensor takes as long as its Python does, so these keep the common case short: checks that
+    # pass are a few attribute reads, messages are made where one fails.
     draws_masks = True      # dropout operators accept a key object in place of a mask tensor
 
     _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
-    @staticmethod
-    def _check_act(what, x, *others, same_shape=True):
-        """Type code of the activation tensor ``x``; every other tensor has to match it."""
-        t = HipBackend._TYPES.get(x.dtype)
+    def _act_type(self, what, x, *others):
+        """Type code of the activation tensor ``x``; every other tensor has to match its type, device and shape."""
+        dt = x.dtype
+        t = self._TYPES.get(dt)
         if t is None:
-            raise _lib.SivError(f"{what}: unsupported dtype {x.dtype} (float32, bfloat16 or float16)")
+            raise _lib.SivError(f"{what}: unsupported dtype {dt} (float32, bfloat16 or float16)")
         if not x.is_cuda:
             raise _lib.SivError(f"{what}: libsiv kernels need tensors on a HIP device (got a CPU tensor); "
                                 "there is no CPU fallback")
         for o in others:
-            if o is None:
-                continue
-            if o.dtype != x.dtype or o.device != x.device:
-                raise _lib.SivError(f"{what}: got {o.dtype} on {o.device} beside {x.dtype} on {x.device}")
-            if same_shape and o.shape != x.shape:
-                raise _lib.SivError(f"{what}: shapes {tuple(o.shape)} and {tuple(x.shape)} differ")
+            if o is not None:
+                if o.dtype != dt or o.get_device() != x.get_device():
+                    raise _lib.SivError(f"{what}: got {o.dtype} on {o.device} beside {dt} on {x.device}")
+                if o.shape != x.shape:
+                    raise _lib.SivError(f"{what}: shapes {tuple(o.shape)} and {tuple(x.shape)} differ")
         return t
 
     @staticmethod
     def _row_extent(what, x):
         """(rows, elements per row): the channels of a voxel for a 5-D tensor, else the last axis."""
-        if x.dim() == 0:
+        sh = x.shape
+        if not sh:
             raise _lib.SivError(f"{what}: needs at least one axis")
-        C = x.shape[1] if x.dim() == 5 else x.shape[-1]
+        C = sh[1] if len(sh) == 5 else sh[-1]
         if C == 0:
             raise _lib.SivError(f"{what}: rows of length 0 have no mean")
         return x.numel() // C, C
@@ -727,41 +739,43 @@ class HipBackend:
                     return x, ld
         return cl(x), C
 
-    @classmethod
-    def _affine(cls, what, x, C, *params):
-        """Type code of weight / bias (fp32, or that of the activations) and the tensors, dense."""
+    def _affine(self, what, x, C, weight, bias):
+        """(type code, weight, bias): fp32 or of the activations' type, both the same, dense; either may be None."""
         dt = None
-        out = []
-        for w in params:
-            if w is not None:
-                if w.device != x.device or w.dtype not in (torch.float32, x.dtype) or (dt or w.dtype) != w.dtype:
-                    raise _lib.SivError(f"{what}: weight and bias must be float32 or {x.dtype}, both the same, on "
-                                        f"{x.device} (got {w.dtype} on {w.device})")
-                if w.numel() != C or w.dim() != 1:
-                    raise _lib.SivError(f"{what}: weight / bias of shape {tuple(w.shape)} for rows of {C}")
-                dt = w.dtype
-                w = w.contiguous()
-            out.append(w)
-        return cls._TYPES[dt or torch.float32], out
+        dev = x.get_device()
+        for w in (weight, bias):
+            if w is None:
+                continue
+            if (w.dtype is not torch.float32 and w.dtype != x.dtype) or (dt or w.dtype) != w.dtype or w.get_device() != dev:
+                raise _lib.SivError(f"{what}: weight and bias must be float32 or {x.dtype}, both the same, on "
+                                    f"{x.device} (got {w.dtype} on {w.device})")
+            if w.dim() != 1 or w.numel() != C:
+                raise _lib.SivError(f"{what}: weight / bias of shape {tuple(w.shape)} for rows of {C}")
+            dt = w.dtype
+        if weight is not None and not weight.is_contiguous():
+            weight = weight.contiguous()
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        return (0 if dt is None else self._TYPES[dt]), weight, bias
 
-    @classmethod
-    def _drop_args(cls, what, x, keep, p):
+    _NO_DROP = (None, 0, 0, None, 0.0)
+
+    def _drop_args(self, what, x, keep, p):
         """(mask pointer or None, seed, stream id, epoch pointer, p) and the tensor that must outlive the launch."""
-        p = float(p)
         if not 0.0 <= p < 1.0:
             raise _lib.SivError(f"{what}: dropout p must lie in [0, 1), got {p}")
         if keep is None:
-            return (None, 0, 0, None, 0.0), None
+            return self._NO_DROP, None
         if torch.is_tensor(keep):
             if keep.dtype != torch.uint8 or keep.shape != x.shape or keep.device != x.device:
                 raise _lib.SivError(f"{what}: the keep mask must be uint8 of shape {tuple(x.shape)} on {x.device}")
             keep = cl(keep)
             return (keep.data_ptr(), 0, 0, None, p), keep
-        m = 2 ** 64 - 1
         e = keep.epoch
         if e is not None and (e.dtype != torch.int64 or e.numel() != 1 or e.device != x.device):
             raise _lib.SivError(f"{what}: the epoch counter of a mask key must be one int64 on {x.device}")
-        return (None, keep.seed & m, keep.stream_id & m, _p(e), p), e
+        m = 0xFFFFFFFFFFFFFFFF
+        return (None, keep.seed & m, keep.stream_id & m, None if e is None else e.data_ptr(), p), e
 
     def _launch(self, what, x, *args):
         """Call the entry point ``what`` on the current stream of x's device, with that device current.  (The raw
@@ -776,46 +790,48 @@ class HipBackend:
         if rc != 0:
             _lib.check(rc, what)
 
-    def _norm_workspace(self, rows, C, t, backward, device):
+    @staticmethod
+    def _norm_scratch(rows, C, t, backward, device):
         """Scratch of one layer-norm call, from torch's allocator (so that it belongs to the stream, or to the
-        graph under capture): (tensor or None, bytes)."""
-        n = ctypes.c_size_t()
-        _lib.check(self.lib.siv_layer_norm_workspace(rows, C, t, backward, ctypes.addressof(n)),
-                   "siv_layer_norm_workspace")
-        return (torch.empty(n.value, dtype=torch.uint8, device=device), n.value) if n.value else (None, 0)
+        graph under capture): (tensor or None, address or None, bytes)."""
+        n = _norm_ws_bytes(rows, C, t, backward)
+        if n == 0:
+            return None, None, 0
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        return ws, ws.data_ptr(), n
 
-    def _affine_targets(self, x, C, pdtype, want_w, want_b, dw_out, db_out):
+    @staticmethod
+    def _affine_targets(x, C, pdtype, want_w, want_b, dw_out, db_out):
         """(dweight, dbias, accumulate): the caller's buffers, or fresh tensors of the parameters' type."""
         if dw_out is not None or db_out is not None:
             for o in (dw_out, db_out):
                 assert o is None or (o.numel() == C and o.is_contiguous() and o.dtype == pdtype)
             return (dw_out if want_w else None), (db_out if want_b else None), 1
-        new = lambda want: torch.empty(C, dtype=pdtype, device=x.device) if want else None
-        return new(want_w), new(want_b), 0
+        dev = x.device
+        return (torch.empty(C, dtype=pdtype, device=dev) if want_w else None,
+                torch.empty(C, dtype=pdtype, device=dev) if want_b else None, 0)
 
     def layer_norm_fwd(self, x, weight, bias, eps: float):
-        what = "layer_norm"
-        t = self._check_act(what, x)
-        rows, C = self._row_extent(what, x)
-        wt, (weight, bias) = self._affine(what, x, C, weight, bias)
+        t = self._act_type("layer_norm", x)
+        rows, C = self._row_extent("layer_norm", x)
+        wt, weight, bias = self._affine("layer_norm", x, C, weight, bias)
         y = like(x)
-        if rows == 0:
-            return y
-        x, ld = self._row_view(x, C)
-        ws, wsb = self._norm_workspace(rows, C, t, 0, x.device)
-        self._launch("siv_layer_norm_fwd", x, x.data_ptr(), ld, _p(weight), _p(bias), wt, eps, y.data_ptr(), t, rows, C,
-                     _p(ws), wsb)
+        if rows:
+            x, ld = self._row_view(x, C)
+            ws, wsp, wsb = self._norm_scratch(rows, C, t, 0, x.device)
+            self._launch("siv_layer_norm_fwd", x, x.data_ptr(), ld, _p(weight), _p(bias), wt, eps, y.data_ptr(), t, rows,
+                         C, wsp, wsb)
         return y
 
     def layer_norm_bwd(self, dy, x, weight, eps: float, pdtype=torch.float32, want_x=True, want_w=True, want_b=True,
                        dw_out=None, db_out=None):
         """(dx, dweight, dbias); ``pdtype``: type of the parameters' gradients.  With ``dw_out`` / ``db_out`` those
         results are ADDED into the buffers."""
-        what = "layer_norm backward"
-        t = self._check_act(what, x, dy)
-        rows, C = self._row_extent(what, x)
-        wt, (weight,) = self._affine(what, x, C, weight)
-        wt = self._TYPES[pdtype] if weight is None else wt
+        t = self._act_type("layer_norm backward", x, dy)
+        rows, C = self._row_extent("layer_norm backward", x)
+        wt, weight, _ = self._affine("layer_norm backward", x, C, weight, None)
+        if weight is None:
+            wt = self._TYPES[pdtype]
         dw, db, acc = self._affine_targets(x, C, pdtype, want_w, want_b, dw_out, db_out)
         dx = like(x) if want_x else None
         if rows == 0:
@@ -823,44 +839,41 @@ class HipBackend:
                 for o in (dw, db):
                     if o is not None:
                         o.zero_()
-            return dx, dw, db
-        if dx is None and dw is None and db is None:
-            return dx, dw, db
-        x, ld = self._row_view(x, C)
-        dy, ldd = self._row_view(dy, C)
-        ws, wsb = self._norm_workspace(rows, C, t, 1, x.device)
-        self._launch("siv_layer_norm_bwd", x, dy.data_ptr(), ldd, x.data_ptr(), ld, _p(weight), wt, eps, _p(dx), _p(dw),
-                     _p(db), acc, t, rows, C, _p(ws), wsb)
+        elif dx is not None or dw is not None or db is not None:
+            x, ld = self._row_view(x, C)
+            dy, ldd = self._row_view(dy, C)
+            ws, wsp, wsb = self._norm_scratch(rows, C, t, 1, x.device)
+            self._launch("siv_layer_norm_bwd", x, dy.data_ptr(), ldd, x.data_ptr(), ld, _p(weight), wt, eps, _p(dx),
+                         _p(dw), _p(db), acc, t, rows, C, wsp, wsb)
         return dx, dw, db
 
     def add_layer_norm_fwd(self, x, residual, keep, p, weight, bias, eps: float):
         """(y, s) with s = residual + dropout(x) and y = layer_norm(s)."""
-        what = "add_layer_norm"
-        t = self._check_act(what, x, residual)
-        rows, C = self._row_extent(what, x)
-        wt, (weight, bias) = self._affine(what, x, C, weight, bias)
-        drop, held = self._drop_args(what, x, keep, p)
+        t = self._act_type("add_layer_norm", x, residual)
+        rows, C = self._row_extent("add_layer_norm", x)
+        wt, weight, bias = self._affine("add_layer_norm", x, C, weight, bias)
+        drop, held = self._drop_args("add_layer_norm", x, keep, p)
         x, residual = cl(x), cl(residual)
         y, s = like(x), like(x)
-        if rows == 0:
-            return y, s
-        ws, wsb = self._norm_workspace(rows, C, t, 0, x.device)
-        self._launch("siv_add_layer_norm_fwd", x, x.data_ptr(), residual.data_ptr(), *drop, _p(weight), _p(bias), wt, eps,
-                     s.data_ptr(), y.data_ptr(), t, rows, C, _p(ws), wsb)
+        if rows:
+            ws, wsp, wsb = self._norm_scratch(rows, C, t, 0, x.device)
+            self._launch("siv_add_layer_norm_fwd", x, x.data_ptr(), residual.data_ptr(), *drop, _p(weight), _p(bias), wt,
+                         eps, s.data_ptr(), y.data_ptr(), t, rows, C, wsp, wsb)
         return y, s
 
     def add_layer_norm_bwd(self, dy, ds, s, keep, p, weight, eps: float, pdtype=torch.float32, want_x=True, want_res=True,
                            want_w=True, want_b=True, dw_out=None, db_out=None):
         """(dx, dresidual, dweight, dbias) from the gradients ``dy`` of y and ``ds`` (or None) of s."""
-        what = "add_layer_norm backward"
-        t = self._check_act(what, s, dy, ds)
-        rows, C = self._row_extent(what, s)
-        wt, (weight,) = self._affine(what, s, C, weight)
-        wt = self._TYPES[pdtype] if weight is None else wt
-        drop, held = self._drop_args(what, s, keep, p)
+        t = self._act_type("add_layer_norm backward", s, dy, ds)
+        rows, C = self._row_extent("add_layer_norm backward", s)
+        wt, weight, _ = self._affine("add_layer_norm backward", s, C, weight, None)
+        if weight is None:
+            wt = self._TYPES[pdtype]
+        drop, held = self._drop_args("add_layer_norm backward", s, keep, p)
         dw, db, acc = self._affine_targets(s, C, pdtype, want_w, want_b, dw_out, db_out)
         dy, s = cl(dy), cl(s)
-        ds = None if ds is None else cl(ds)
+        if ds is not None:
+            ds = cl(ds)
         both = keep is None and want_x and want_res         # nothing dropped: the two gradients are one tensor
         dres = like(s) if want_res else None
         dx = like(s) if want_x and not both else None
@@ -869,34 +882,36 @@ class HipBackend:
                 for o in (dw, db):
                     if o is not None:
                         o.zero_()
-        elif not (dx is None and dres is None and dw is None and db is None):
-            ws, wsb = self._norm_workspace(rows, C, t, 1, s.device)
+        elif dx is not None or dres is not None or dw is not None or db is not None:
+            ws, wsp, wsb = self._norm_scratch(rows, C, t, 1, s.device)
             self._launch("siv_add_layer_norm_bwd", s, dy.data_ptr(), _p(ds), s.data_ptr(), *drop, _p(weight), wt, eps,
-                         _p(dx), _p(dres), _p(dw), _p(db), acc, t, rows, C, _p(ws), wsb)
+                         _p(dx), _p(dres), _p(dw), _p(db), acc, t, rows, C, wsp, wsb)
         return (dres if both else dx), dres, dw, db
 
     def dropout_fwd(self, x, keep, p, slope: float = 1.0, residual=None):
         """[residual +] dropout(LeakyReLU_slope(x)); slope 1 = no activation."""
-        what = "dropout"
-        t = self._check_act(what, x, residual)
-        drop, held = self._drop_args(what, x, keep, p)
+        t = self._act_type("dropout", x, residual)
+        drop, held = self._drop_args("dropout", x, keep, p)
         x = cl(x)
-        residual = None if residual is None else cl(residual)
+        if residual is not None:
+            residual = cl(residual)
         out = like(x)
-        if x.numel():
-            self._launch("siv_dropout_fwd", x, x.data_ptr(), _p(residual), *drop, slope, out.data_ptr(), t, x.numel())
+        n = x.numel()
+        if n:
+            self._launch("siv_dropout_fwd", x, x.data_ptr(), _p(residual), *drop, slope, out.data_ptr(), t, n)
         return out
 
     def dropout_bwd(self, dout, x, keep, p, slope: float = 1.0):
         """Gradient of x; ``x`` may be None where slope == 1."""
-        what = "dropout backward"
-        t = self._check_act(what, dout, x)
-        drop, held = self._drop_args(what, dout, keep, p)
+        t = self._act_type("dropout backward", dout, x)
+        drop, held = self._drop_args("dropout backward", dout, keep, p)
         dout = cl(dout)
-        x = None if x is None else cl(x)
+        if x is not None:
+            x = cl(x)
         dx = like(dout)
-        if dout.numel():
-            self._launch("siv_dropout_bwd", dout, dout.data_ptr(), _p(x), *drop, slope, dx.data_ptr(), t, dout.numel())
+        n = dout.numel()
+        if n:
+            self._launch("siv_dropout_bwd", dout, dout.data_ptr(), _p(x), *drop, slope, dx.data_ptr(), t, n)
         return dx
 
     # ---- latent sampling and losses ------------------------------------------------

@@ -4,6 +4,7 @@ backward passes run is decided by ``requires_grad`` / ``detach`` exactly as in t
 reference trainer)."""
 from __future__ import annotations
 
+import functools
 import os
 from typing import Optional
 
@@ -618,6 +619,16 @@ def draws_masks() -> bool:
     return getattr(get_backend(), "draws_masks", False)
 
 
+def _first_order(backward):
+    """``backward`` without a derivative of its own (once_differentiable); where none is asked for, called directly."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _mask_of(keep):
     """(mask tensor or None, key or None): the two places a dropout mask can come from."""
     return (keep, None) if torch.is_tensor(keep) else (None, keep)
@@ -632,7 +643,7 @@ class _Dropout(Function):
         return get_backend().dropout_fwd(x, keep, p, slope, residual)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         dx = None
         if ctx.needs_input_grad[0]:
@@ -646,6 +657,8 @@ def dropout(x, keep, p: float, residual=None):
     ``keep``: a ``rng.PhiloxKeep`` key (``rng.get_rng().keep_mask_key(x.shape, p, x.device)``), whose mask is drawn by
     the kernels, forward and backward, and never stored; a uint8 mask tensor; or None (nothing dropped).  A dropped
     element contributes 0 whatever ``x`` holds there.  float32, bfloat16 or float16, any shape."""
+    if not torch.is_grad_enabled():
+        return get_backend().dropout_fwd(x, keep, p, 1.0, residual)
     return _Dropout.apply(x, residual, keep, p, 1.0)
 
 
@@ -659,7 +672,7 @@ class _LayerNorm(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -689,6 +702,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     ``(x - mean) / sqrt(var + eps) * weight + bias`` with the row's own mean and biased variance -- no batch, no running
     statistics.  float32, bfloat16 or float16; ``weight`` / ``bias`` float32 or of x's type, or None.  Rows may be slices
     of wider rows.  Statistics are fp32 and formed again by the backward pass; only ``x`` is kept."""
+    if not torch.is_grad_enabled():
+        return get_backend().layer_norm_fwd(x, weight, bias, eps)
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
@@ -704,7 +719,7 @@ class _AddLayerNorm(Function):
         return y, s
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, ds):
         s, weight, mask = ctx.saved_tensors
         eps, p, pdtype = ctx.cfg
@@ -727,6 +742,8 @@ def add_layer_norm(x, residual, weight=None, bias=None, eps: float = 1e-5, keep=
     """The closing step of a residual branch in one pass: ``s = residual + dropout(x)`` and ``y = layer_norm(s)``;
     returns ``(y, s)``.  ``keep`` / ``p`` as in ``dropout``, rows and parameters as in ``layer_norm``; ``s`` is held in
     the tensors' type and it is what is normalised."""
+    if not torch.is_grad_enabled():
+        return get_backend().add_layer_norm_fwd(x, residual, keep, p, weight, bias, eps)
     return _AddLayerNorm.apply(x, residual, weight, bias, eps, keep, p)
 
 
