@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SIV_LIB", os.path.join(_HERE, "libsiv.so"))   # SIV_LIB: A/B builds of the library
@@ -141,6 +142,21 @@ def load() -> C.CDLL:
     lib.siv_workspace_bytes.argtypes = []
     _lib = lib
     return lib
+
+
+def load_nodes(lib: C.CDLL):
+    """The extension module with the autograd nodes of the layer-norm and dropout operators (csrc/torch_nodes.cpp), bound
+    to the entry points of ``lib``; None, with a warning, where it was not built (the same operators then run through
+    Python autograd functions)."""
+    try:
+        from . import _siv_torch
+    except ImportError as e:
+        warnings.warn(f"siv: autograd nodes not available ({e}); small layer-norm and dropout calls will be slower")
+        return None
+    names = ("siv_layer_norm_workspace", "siv_layer_norm_fwd", "siv_layer_norm_bwd", "siv_add_layer_norm_fwd",
+             "siv_add_layer_norm_bwd", "siv_dropout_fwd", "siv_dropout_bwd", "siv_last_error")
+    _siv_torch.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names})
+    return _siv_torch
 
 
 def check(rc: int, what: str) -> None:

@@ -52,6 +52,7 @@ class HipBackend:
 
     def __init__(self):
         self.lib = _lib.load()
+        self.nodes = _lib.load_nodes(self.lib)      # autograd nodes of layer_norm / add_layer_norm / dropout, or None
         self._ws = {}
         self._side = {}
         self._pack_cache = {}          # device -> donated cache memory
@@ -681,8 +682,7 @@ class HipBackend:
         return dx
 
     # ---- layer normalisation, dropout without a stored mask (fp32, bf16, fp16) --------------------------
-    # A call on a small tensor takes as long as its Python does, so these keep the common case short: checks that
-    # pass are a few attribute reads, messages are made where one fails.
+    # What siv.ops runs where ``nodes`` does not take a call: every layout, and the words of every refusal.
     draws_masks = True      # dropout operators accept a key object in place of a mask tensor
 
     _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

@@ -10,7 +10,6 @@ from typing import Optional
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import activations
 from .backend import get_backend
@@ -610,7 +609,7 @@ def act_dropout(x, slope: float, keep=None, p: float = 0.0):
     ``rng.PhiloxKeep`` key (``draws_masks()``): the kernels then draw the mask themselves, forward and backward, and no
     mask tensor exists."""
     if keep is not None and not torch.is_tensor(keep):
-        return _Dropout.apply(x, None, keep, p, slope)
+        return _dropout(x, None, keep, p, slope)
     return _ActDropout.apply(x, keep, p, slope)
 
 
@@ -619,14 +618,34 @@ def draws_masks() -> bool:
     return getattr(get_backend(), "draws_masks", False)
 
 
-def _first_order(backward):
-    """``backward`` without a derivative of its own (once_differentiable); where none is asked for, called directly."""
-    guarded = once_differentiable(backward)
+class _NoSecondDerivative(Function):
+    """A gradient under create_graph, tied to what it was computed from: asking for its derivative raises."""
 
-    @functools.wraps(backward)
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
+    @staticmethod
+    def forward(ctx, grad, what, *sources):
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"the backward pass of {ctx.what} is not differentiable")
+
+
+def _first_order(what):
+    """Decorator of a ``backward`` that has no derivative of its own."""
+    def wrap(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            if not torch.is_grad_enabled():
+                return backward(ctx, *grads)
+            with torch.no_grad():
+                outs = backward(ctx, *grads)
+            sources = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad]
+            if not sources:
+                return outs
+            return tuple(None if o is None else _NoSecondDerivative.apply(o, what, *sources) for o in outs)
+        return run
+    return wrap
 
 
 def _mask_of(keep):
@@ -643,7 +662,7 @@ class _Dropout(Function):
         return get_backend().dropout_fwd(x, keep, p, slope, residual)
 
     @staticmethod
-    @_first_order
+    @_first_order("dropout")
     def backward(ctx, dout):
         dx = None
         if ctx.needs_input_grad[0]:
@@ -652,14 +671,36 @@ class _Dropout(Function):
         return dx, (dout if ctx.needs_input_grad[1] else None), None, None, None
 
 
+def _nodes():
+    """The native autograd nodes (siv/_siv_torch), or None.  They answer None to a call that is not theirs: other
+    layouts than dense rows, another device than the current one, arguments to be refused."""
+    return getattr(get_backend(), "nodes", None)
+
+
+def _mask_fields(keep):
+    """(mask tensor, seed, stream id, epoch) of a mask tensor, a key, or None, as the nodes take them."""
+    if keep is None:
+        return None, None, None, None
+    if torch.is_tensor(keep):
+        return keep, None, None, None
+    return None, keep.seed, keep.stream_id, keep.epoch
+
+
+def _dropout(x, residual, keep, p, slope):
+    nodes = _nodes()
+    if nodes is not None:
+        out = nodes.dropout(x, residual, *_mask_fields(keep), p, slope)
+        if out is not None:
+            return out
+    return _Dropout.apply(x, residual, keep, p, slope)
+
+
 def dropout(x, keep, p: float, residual=None):
     """nn.Dropout(p) with its mask given: ``x * keep / (1 - p)``, onto ``residual`` where one is given, in one pass.
     ``keep``: a ``rng.PhiloxKeep`` key (``rng.get_rng().keep_mask_key(x.shape, p, x.device)``), whose mask is drawn by
     the kernels, forward and backward, and never stored; a uint8 mask tensor; or None (nothing dropped).  A dropped
     element contributes 0 whatever ``x`` holds there.  float32, bfloat16 or float16, any shape."""
-    if not torch.is_grad_enabled():
-        return get_backend().dropout_fwd(x, keep, p, 1.0, residual)
-    return _Dropout.apply(x, residual, keep, p, 1.0)
+    return _dropout(x, residual, keep, p, 1.0)
 
 
 class _LayerNorm(Function):
@@ -672,7 +713,7 @@ class _LayerNorm(Function):
         return y
 
     @staticmethod
-    @_first_order
+    @_first_order("layer_norm")
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -702,8 +743,11 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     ``(x - mean) / sqrt(var + eps) * weight + bias`` with the row's own mean and biased variance -- no batch, no running
     statistics.  float32, bfloat16 or float16; ``weight`` / ``bias`` float32 or of x's type, or None.  Rows may be slices
     of wider rows.  Statistics are fp32 and formed again by the backward pass; only ``x`` is kept."""
-    if not torch.is_grad_enabled():
-        return get_backend().layer_norm_fwd(x, weight, bias, eps)
+    nodes = _nodes()
+    if nodes is not None:
+        y = nodes.layer_norm(x, weight, bias, eps, _grad_buf(weight), _grad_buf(bias))
+        if y is not None:
+            return y
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
@@ -719,7 +763,7 @@ class _AddLayerNorm(Function):
         return y, s
 
     @staticmethod
-    @_first_order
+    @_first_order("add_layer_norm")
     def backward(ctx, dy, ds):
         s, weight, mask = ctx.saved_tensors
         eps, p, pdtype = ctx.cfg
@@ -742,8 +786,12 @@ def add_layer_norm(x, residual, weight=None, bias=None, eps: float = 1e-5, keep=
     """The closing step of a residual branch in one pass: ``s = residual + dropout(x)`` and ``y = layer_norm(s)``;
     returns ``(y, s)``.  ``keep`` / ``p`` as in ``dropout``, rows and parameters as in ``layer_norm``; ``s`` is held in
     the tensors' type and it is what is normalised."""
-    if not torch.is_grad_enabled():
-        return get_backend().add_layer_norm_fwd(x, residual, keep, p, weight, bias, eps)
+    nodes = _nodes()
+    if nodes is not None:
+        ys = nodes.add_layer_norm(x, residual, weight, bias, eps, *_mask_fields(keep), p, _grad_buf(weight),
+                                  _grad_buf(bias))
+        if ys is not None:
+            return ys
     return _AddLayerNorm.apply(x, residual, weight, bias, eps, keep, p)
 
 

@@ -11,11 +11,18 @@ pytestmark = pytest.mark.gpu
 CL3D = torch.channels_last_3d
 
 
-@pytest.fixture(autouse=True)
-def hip():
+@pytest.fixture(autouse=True, params=["nodes", "python"])
+def hip(request):
+    """The backend, with its native autograd nodes and with the Python autograd functions only."""
     import siv.backend as sb
     sb.set_backend(None)
-    return sb.get_backend()
+    b = sb.get_backend()
+    nodes = b.nodes
+    assert nodes is not None, "siv/_siv_torch.so is not built"
+    if request.param == "python":
+        b.nodes = None
+    yield b
+    b.nodes = nodes
 
 
 def ops():
@@ -237,10 +244,72 @@ def test_refusals(hip):
                       (lambda: o.add_layer_norm(x, x[:2]), "shapes")):
         with pytest.raises(SivError, match=word):
             bad()
-    xg = torch.zeros(4, 8, device="cuda", requires_grad=True)
-    dx, = torch.autograd.grad(o.layer_norm(xg).sum(), xg, create_graph=True)
-    with pytest.raises(RuntimeError):           # no second derivative: an error, not a zero
-        torch.autograd.grad(dx.sum(), xg)
+    # no second derivative: an error, not a zero, also where another path leads to the same leaf
+    xg = rnd(1, 4, 8).cuda().requires_grad_()
+    for f in (lambda: o.layer_norm(xg), lambda: o.add_layer_norm(xg, xg, keep=key(), p=0.5)[0],
+              lambda: o.dropout(xg, key(), 0.5).square()):
+        first, = torch.autograd.grad(f().sum(), xg)
+        dx, = torch.autograd.grad(f().sum(), xg, create_graph=True)
+        assert torch.equal(dx, first)
+        with pytest.raises(RuntimeError, match="differentia"):
+            torch.autograd.grad((dx * xg.sin()).sum(), xg)
+    dx, = torch.autograd.grad(o.dropout(xg, key(), 0.5).sum(), xg, create_graph=True)      # does not depend on xg
+    assert torch.equal(torch.autograd.grad((dx * xg.sin()).sum(), xg)[0], dx.detach() * xg.detach().cos())
+
+
+def test_gradients_that_are_not_dense(hip):
+    """Upstream gradients as autograd hands them on: expanded, transposed, strided."""
+    o = ops()
+    x, w, b = rnd(1, 12, 40).cuda().requires_grad_(), torch.ones(40, device="cuda", requires_grad=True), None
+    ups = (torch.ones((), device="cuda").expand(12, 40), rnd(2, 40, 12).cuda().t(), rnd(3, 12, 90).cuda()[:, 5:45],
+           rnd(4, 24, 80).cuda()[::2, ::2])
+    for dy in ups:
+        for f in (lambda: o.layer_norm(x, w), lambda: o.add_layer_norm(x, x.detach(), w, keep=key(), p=0.5)[0],
+                  lambda: o.add_layer_norm(x, x.detach(), w, keep=key(), p=0.5)[1], lambda: o.dropout(x, key(), 0.5),
+                  lambda: o.act_dropout(x, 0.2, key(), 0.5)):
+            got = torch.autograd.grad(f(), (x, w), dy, allow_unused=True)
+            want = torch.autograd.grad(f(), (x, w), dy.contiguous(), allow_unused=True)
+            assert all(a is c or torch.equal(a, c) for a, c in zip(got, want))
+    v = rnd(5, 2, 6, 3, 4, 5).cuda().contiguous(memory_format=CL3D).requires_grad_()
+    dy = rnd(6, 2, 6, 3, 4, 5).cuda()                      # NCDHW memory
+    for f in (lambda: o.layer_norm(v), lambda: o.dropout(v, key(), 0.5), lambda: o.add_layer_norm(v, v.detach())[0]):
+        got, = torch.autograd.grad(f(), v, dy)
+        want, = torch.autograd.grad(f(), v, dy.contiguous(memory_format=CL3D))
+        assert torch.equal(got, want)
+
+
+def test_a_changed_input_is_noticed(hip):
+    """The kept input written between forward and backward: an error, as for torch's own operators."""
+    o = ops()
+    x = rnd(1, 4, 8).cuda().requires_grad_()
+    for f in (lambda t: o.layer_norm(t), lambda t: o.act_dropout(t, 0.0, key(), 0.5)):
+        t = x * 1.0
+        y = f(t)
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.sum().backward()
+    y, s = o.add_layer_norm(x, x.detach())
+    s.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+def test_frozen_parameters_and_inputs(hip):
+    """Only what requires a gradient gets one; parameters that are frozen stay as they are."""
+    o = ops()
+    x, w, b = rnd(1, 12, 40).cuda(), torch.ones(40, device="cuda"), torch.zeros(40, device="cuda")
+    full = [t.clone().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(o.layer_norm(*full), full, torch.ones(12, 40, device="cuda"))
+    for mask in range(1, 8):
+        ts = [t.clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((x, w, b))]
+        y = o.layer_norm(*ts)
+        y.backward(torch.ones(12, 40, device="cuda"))
+        for i, t in enumerate(ts):
+            assert (t.grad is None) == (not mask >> i & 1)
+            assert t.grad is None or torch.equal(t.grad, want[i])
+    assert not o.layer_norm(x, w, b).requires_grad and not o.dropout(x, key(), 0.5).requires_grad
+    with torch.no_grad():
+        assert not o.layer_norm(*full).requires_grad
 
 
 # ---- dropout ----------------------------------------------------------------------------------------------------------
