@@ -25,6 +25,24 @@ struct alignas(16) Pack {
     static constexpr int N = 16 / sizeof(T);
     T e[N];
 };
+// A result that nothing in the call reads again: stored non-temporally, so that it leaves the L2 (which a kernel's end
+// writes back anyway) to the operands.
+template <typename T>
+__device__ __forceinline__ void store_stream(T* p, const Pack<T>& v) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    words w;
+    __builtin_memcpy(&w, v.e, 16);
+    __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
+}
+// An operand that nothing is expected to read again soon.
+template <typename T>
+__device__ __forceinline__ Pack<T> load_stream(const T* p) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    const words w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
+    Pack<T> v;
+    __builtin_memcpy(v.e, &w, 16);
+    return v;
+}
 // `have` elements of the row are left at p (<= 0: none, the pack is zero; >= N: a whole one).  AL: p is 16-byte
 // aligned and have is a multiple of N.  Otherwise p has the element's alignment only: the hardware takes a 16-byte
 // access at any address, so whole packs still are one instruction.
@@ -49,7 +67,7 @@ template <bool AL, typename T>
 __device__ __forceinline__ void store_pack(T* p, long have, const Pack<T>& v) {
     constexpr int N = Pack<T>::N;
     if (AL) {
-        if (have > 0) *reinterpret_cast<Pack<T>*>(p) = v;
+        if (have > 0) store_stream(p, v);
     } else if (have >= N) {
         __builtin_memcpy(p, v.e, 16);
     } else {
@@ -91,8 +109,15 @@ __device__ __forceinline__ uint64_t drop_sid(const Drop& d) {
 // Words of elements i .. i+N-1 of a stored mask, of which the first `have` exist.
 template <int N>
 __device__ __forceinline__ void stored_words(const Drop& d, uint64_t i, long have, uint32_t (&w)[N]) {
+    if (have >= N) {
+        uint8_t m[N];
+        __builtin_memcpy(m, d.keep + i, N);
 #pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = (j < have && d.keep[i + j]) ? ~0u : 0u;
+        for (int j = 0; j < N; ++j) w[j] = m[j] ? ~0u : 0u;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = (j < have && d.keep[i + j]) ? ~0u : 0u;
+    }
 }
 // The same drawn.  QUAD: i is a multiple of 4, so the N elements are whole Philox calls; otherwise one call more and a
 // shift by 0 to 3 words.

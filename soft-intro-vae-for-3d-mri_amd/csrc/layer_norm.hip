@@ -5,6 +5,7 @@
 // The mean is summed twice: m0 = sum x / C, then d = x - m0, delta = sum d / C, var = sum d^2 / C - delta^2.  x - m0
 // is exact or nearly so, and delta takes back the rounding of m0, so rows far off zero keep their deviations.
 // The backward pass forms the statistics again from the row it reads anyway, so forward leaves nothing behind.
+#include <algorithm>
 #include "elem_types.h"
 
 namespace siv {
@@ -53,58 +54,128 @@ __device__ __forceinline__ void lanes_sum(float (&v)[N], int lg) {
              v[k] = __uint_as_float(t[0]) + __uint_as_float(t[1]))
 #undef SIV_STEP
 }
-// Sums over the lanes that share a row: part of a wave, or (BLK) a block of 256.  Two LDS buffers in turn: the barrier
-// of one sum also separates the readers of the sum before it from the writers of the next.
-template <bool BLK>
+// Sums over the lanes that share a row: part of a wave (NT = 64), or a block of NT.  Two LDS buffers in turn: the
+// barrier of one sum also separates the readers of the sum before it from the writers of the next.
+template <int NT>
 struct RowSum {
-    float (*sh)[4][4];
+    float4 (*sh)[NT / 64];
     int lg, turn;
     template <int N>
     __device__ __forceinline__ void operator()(float (&v)[N]) {
-        if (!BLK) {
+        if (NT == 64) {
             lanes_sum(v, lg);
             return;
         }
         lanes_sum(v, 6);
-        const int w = threadIdx.x >> 6;
+        float4* buf = sh[turn];
         if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int k = 0; k < N; ++k) sh[turn][w][k] = v[k];
+            buf[threadIdx.x >> 6] = make_float4(v[0], N > 1 ? v[N > 1 ? 1 : 0] : 0.f, N > 2 ? v[N > 2 ? 2 : 0] : 0.f,
+                                                N > 3 ? v[N > 3 ? 3 : 0] : 0.f);
         __syncthreads();
+        float4 s = buf[0];
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = (sh[turn][0][k] + sh[turn][1][k]) + (sh[turn][2][k] + sh[turn][3][k]);
+        for (int w = 1; w < NT / 64; ++w) {
+            const float4 o = buf[w];
+            s.x += o.x;
+            if (N > 1) s.y += o.y;
+            if (N > 2) s.z += o.z;
+            if (N > 3) s.w += o.w;
+        }
+        v[0] = s.x;
+        if (N > 1) v[N > 1 ? 1 : 0] = s.y;
+        if (N > 2) v[N > 2 ? 2 : 0] = s.z;
+        if (N > 3) v[N > 3 ? 3 : 0] = s.w;
         turn ^= 1;
     }
 };
 
-// N consecutive parameters from column c on (have of them exist; the rest 0)
-template <bool AL, typename T, int N>
-__device__ __forceinline__ void load_params(const void* w, int f32, long c, long have, float dflt, float (&out)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) out[j] = dflt;
-    if (!w) return;
-    if (f32) {
-        const float* p = (const float*)w + c;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (AL ? have > 0 : j < have) out[j] = p[j];
-    } else {
-        const T* p = (const T*)w + c;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (AL ? have > 0 : j < have) out[j] = (float)p[j];
+// ---- the columns of a lane's pack ------------------------------------------------------------------------------------
+// ALIGNED: rows start on 16 bytes and hold whole packs.  OVERLAP: they need not; the last pack of a row is moved back so
+// that it ends with the row, the columns it shares with the pack before it count there only (both store the same
+// value).  Every access is one 16-byte instruction either way.  SHORT: rows of less than a pack, element by element.
+enum Cols { SHORT, OVERLAP, ALIGNED };
+template <typename T, int COLS>
+struct Span {
+    static constexpr int N = Pack<T>::N;
+    long c;                 // first column accessed
+    int lo, hi;             // elements lo .. hi-1 of the pack are this lane's
+    __device__ __forceinline__ Span() {}
+    template <int OTHER>
+    __device__ __forceinline__ explicit Span(const Span<T, OTHER>& o) : c(o.c), lo(o.lo), hi(o.hi) {}
+    __device__ __forceinline__ Span(long pack, long C) {
+        c = pack * N;
+        const long have = C - c;
+        lo = 0;
+        hi = have >= N ? N : have > 0 ? (int)have : 0;
+        if (COLS == OVERLAP && have < N) {
+            lo = have > 0 ? N - (int)have : N;
+            hi = N;
+            c = C - N;
+        }
     }
-}
+    __device__ __forceinline__ bool any() const { return lo < hi; }
+    __device__ __forceinline__ bool mine(int j) const {
+        return COLS == ALIGNED ? hi > 0 : COLS == OVERLAP ? j >= lo : j < hi;
+    }
+    // does the access touch element j (a column of the row)
+    __device__ __forceinline__ bool touches(int j) const { return COLS == SHORT ? j < hi : any(); }
+    // LAST: nothing is expected to read the tensor again soon
+    template <bool LAST = false>
+    __device__ __forceinline__ Pack<T> load(const void* row, bool ok) const {
+        Pack<T> v;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v.e[j] = (T)0.f;
+        if (!ok || !any()) return v;
+        const T* p = (const T*)row + c;
+        if (COLS == ALIGNED) v = LAST ? load_stream(p) : *reinterpret_cast<const Pack<T>*>(p);
+        else if (COLS == OVERLAP) __builtin_memcpy(v.e, p, 16);
+        else
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < hi) v.e[j] = p[j];
+        return v;
+    }
+    __device__ __forceinline__ void store(void* row, bool ok, const Pack<T>& v) const {
+        if (!ok || !any()) return;
+        T* p = (T*)row + c;
+        if (COLS == ALIGNED) store_stream(p, v);
+        else if (COLS == OVERLAP) __builtin_memcpy(p, v.e, 16);
+        else
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < hi) p[j] = v.e[j];
+    }
+    // this pack's columns of a parameter vector, in as few loads as the type allows
+    __device__ __forceinline__ void params(const void* w, int f32, float dflt, float (&out)[N]) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = dflt;
+        if (!w || !any()) return;
+        if (f32) {
+            const float* p = (const float*)w + c;
+            if (COLS == SHORT) {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (j < hi) out[j] = p[j];
+            } else {
+                __builtin_memcpy(out, p, 4 * N);
+            }
+        } else {
+            const Pack<T> v = Span<T, COLS == SHORT ? SHORT : OVERLAP>(*this).load(w, true);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (COLS != SHORT || j < hi) out[j] = (float)v.e[j];
+        }
+    }
+};
 template <typename T>
 __device__ __forceinline__ void put_param(void* out, int f32, long c, float v, int accumulate) {
     if (f32) ((float*)out)[c] = accumulate ? ((float*)out)[c] + v : v;
     else ((T*)out)[c] = (T)(accumulate ? (float)((T*)out)[c] + v : v);
 }
 
-// residual + dropout(x) of one pack, as it is held
-template <typename T, bool AL>
-__device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res, const Drop& d, uint64_t sid, long i,
-                                            long have) {
+// residual + dropout(x) of one pack from element i on, as it is held
+template <typename T, int COLS>
+__device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res, const Drop& d, uint64_t sid, long i, int hi) {
     constexpr int N = Pack<T>::N;
     Pack<T> s;
     if (d.mode == 0) {
@@ -113,56 +184,63 @@ __device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res
         return s;
     }
     uint32_t w[N];
-    drop_words<N, AL>(d, sid, i, have, w);
+    drop_words<N, COLS == ALIGNED>(d, sid, i, hi, w);
 #pragma unroll
     for (int j = 0; j < N; ++j) s.e[j] = (T)((float)res.e[j] + (w[j] >= d.least ? (float)x.e[j] * d.scale : 0.f));
     return s;
 }
 
 // ---- rows held in registers -----------------------------------------------------------------------------------------
-// A row is spread over 2^lg lanes of a wave, 64 >> lg rows to a wave (wave form), or over the 256 threads of a block
-// (BLK); a lane holds NV packs of 16 bytes.  One pass over the data; blocks walk the rows in strides of the grid, so
-// that weights and the parameters' gradients stay in registers.
-template <typename T, int NV, bool BLK, bool AL, bool RES>
-__global__ __launch_bounds__(256) void ln_fwd_k(NormArgs a, Drop d) {
+// A row is spread over 2^lg lanes of a wave, 64 >> lg rows to a wave and four waves to a block (NT = 64), or over the
+// NT threads of a block; a lane holds NV packs of 16 bytes.  One pass over the data.  Blocks walk the rows in strides of
+// the grid, so that weights and the parameters' gradients stay in registers; the next row is requested before the
+// present one is worked on.
+template <typename T, int NV, int NT, int COLS, bool RES>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_fwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
-    __shared__ float sh[2][4][4];
-    RowSum<BLK> row_sum{sh, a.lg, 0};
+    constexpr bool AHEAD = NV > 1 || NT > 64;
+    __shared__ float4 sh[2][NT / 64];
+    RowSum<NT> row_sum{sh, a.lg, 0};
     const int lane = threadIdx.x & 63;
-    const int G = BLK ? 256 : 1 << a.lg;
-    const int sub = BLK ? threadIdx.x : lane & (G - 1);
-    const long per = BLK ? 1 : 256 >> a.lg;                           // rows of one block step
-    const long first = BLK ? 0 : threadIdx.x >> a.lg;
+    const int G = NT == 64 ? 1 << a.lg : NT;
+    const int sub = NT == 64 ? lane & (G - 1) : threadIdx.x;
+    const long per = NT == 64 ? 256 >> a.lg : 1;                      // rows of one block step
+    const long step = (long)gridDim.x * per;
     const uint64_t sid = RES ? drop_sid(d) : 0;
     const float invC = 1.0f / (float)a.C;
-    long have[NV];
+    Span<T, COLS> sp[NV];
     float w[NV][N], b[NV][N];
+    long row = (long)blockIdx.x * per + (NT == 64 ? threadIdx.x >> a.lg : 0);
+    Pack<T> x[NV], q[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const long c = (long)(k * G + sub) * N;
-        have[k] = a.C - c;
-        load_params<AL, T>(a.weight, a.wf32, c, have[k], 1.f, w[k]);
-        load_params<AL, T>(a.bias, a.wf32, c, have[k], 0.f, b[k]);
+        sp[k] = Span<T, COLS>(k * G + sub, a.C);
+        x[k] = sp[k].load((const T*)a.x + row * a.ldx, row < a.rows);
+        if (RES) q[k] = sp[k].load((const T*)a.res + row * a.C, row < a.rows);
+        sp[k].params(a.weight, a.wf32, 1.f, w[k]);
+        sp[k].params(a.bias, a.wf32, 0.f, b[k]);
     }
-    for (long row0 = (long)blockIdx.x * per; row0 < a.rows; row0 += (long)gridDim.x * per) {
-        const long row = row0 + first;
-        const bool ok = row < a.rows;
+    // (the block's first row decides: every lane of a block makes the same number of steps)
+    for (long lead = (long)blockIdx.x * per; lead < a.rows; lead += step, row += step) {
+        const bool ok = row < a.rows, more = row + step < a.rows;
+        Pack<T> xn[NV], qn[NV];
+        if (AHEAD)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                xn[k] = sp[k].load((const T*)a.x + (row + step) * a.ldx, more);
+                if (RES) qn[k] = sp[k].load((const T*)a.res + (row + step) * a.C, more);
+            }
         float v[NV][N];
         float s1[1] = {0.f};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const long c = (long)(k * G + sub) * N;
-            const long hv = ok ? have[k] : 0;
-            Pack<T> p = load_pack<AL>((const T*)a.x + row * a.ldx + c, hv);
             if (RES) {
-                const long i = row * a.C + c;
-                const Pack<T> q = load_pack<AL>((const T*)a.res + i, hv);
-                if (hv > 0) p = add_drop<T, AL>(p, q, d, sid, i, hv);
-                store_pack<AL>((T*)a.s + i, hv, p);
+                if (ok && sp[k].any()) x[k] = add_drop<T, COLS>(x[k], q[k], d, sid, row * a.C + sp[k].c, sp[k].hi);
+                sp[k].store((T*)a.s + row * a.C, ok, x[k]);
             }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                v[k][j] = (AL || j < hv) ? (float)p.e[j] : 0.f;
+                v[k][j] = sp[k].mine(j) ? (float)x[k].e[j] : 0.f;
                 s1[0] += v[k][j];
             }
         }
@@ -173,9 +251,10 @@ __global__ __launch_bounds__(256) void ln_fwd_k(NormArgs a, Drop d) {
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                v[k][j] = (AL ? have[k] > 0 : j < have[k]) ? v[k][j] - m0 : 0.f;
-                m[0] += v[k][j];
-                m[1] += v[k][j] * v[k][j];
+                v[k][j] = (float)x[k].e[j] - m0;
+                const float t = sp[k].mine(j) ? v[k][j] : 0.f;
+                m[0] += t;
+                m[1] += t * t;
             }
         row_sum(m);
         const float delta = m[0] * invC;
@@ -185,68 +264,71 @@ __global__ __launch_bounds__(256) void ln_fwd_k(NormArgs a, Drop d) {
             Pack<T> p;
 #pragma unroll
             for (int j = 0; j < N; ++j) p.e[j] = (T)((v[k][j] - delta) * r * w[k][j] + b[k][j]);
-            store_pack<AL>((T*)a.y + row * a.C + (long)(k * G + sub) * N, ok ? have[k] : 0, p);
+            sp[k].store((T*)a.y + row * a.C, ok, p);
+            x[k] = AHEAD ? xn[k] : sp[k].load((const T*)a.x + (row + step) * a.ldx, more);
+            if (RES) q[k] = AHEAD ? qn[k] : sp[k].load((const T*)a.res + (row + step) * a.C, more);
         }
     }
 }
 
 // The same rows backward.  Each lane sums dy h and dy of its columns over the rows it sees; a block's sums go to
 // a.part, or straight to the results where there is one block.
-template <typename T, int NV, bool BLK, bool AL>
-__global__ __launch_bounds__(256) void ln_bwd_k(NormArgs a, Drop d) {
+template <typename T, int NV, int NT, int COLS>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_bwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
-    __shared__ float sh[2][4][4];
-    __shared__ float fold[BLK ? 1 : 4 * 64 * NV * N];
-    RowSum<BLK> row_sum{sh, a.lg, 0};
+    constexpr bool LAST = NT == 64;
+    __shared__ float4 sh[2][NT / 64];
+    __shared__ float fold[NT == 64 ? 4 * 64 * NV * N : 1];
+    RowSum<NT> row_sum{sh, a.lg, 0};
     const int lane = threadIdx.x & 63;
-    const int G = BLK ? 256 : 1 << a.lg;
-    const int sub = BLK ? threadIdx.x : lane & (G - 1);
-    const long per = BLK ? 1 : 256 >> a.lg;
-    const long first = BLK ? 0 : threadIdx.x >> a.lg;
+    const int G = NT == 64 ? 1 << a.lg : NT;
+    const int sub = NT == 64 ? lane & (G - 1) : threadIdx.x;
+    const long per = NT == 64 ? 256 >> a.lg : 1;
+    const long step = (long)gridDim.x * per;
     const uint64_t sid = drop_sid(d);
     const float invC = 1.0f / (float)a.C;
-    long have[NV];
+    Span<T, COLS> sp[NV];
     float w[NV][N], gw[NV][N], gb[NV][N];
+    long row = (long)blockIdx.x * per + (NT == 64 ? threadIdx.x >> a.lg : 0);
+    Pack<T> x[NV], gy[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const long c = (long)(k * G + sub) * N;
-        have[k] = a.C - c;
-        load_params<AL, T>(a.weight, a.wf32, c, have[k], 1.f, w[k]);
+        sp[k] = Span<T, COLS>(k * G + sub, a.C);
+        x[k] = sp[k].template load<LAST>((const T*)a.x + row * a.ldx, row < a.rows);
+        gy[k] = sp[k].template load<LAST>((const T*)a.dy + row * a.lddy, row < a.rows);
+        sp[k].params(a.weight, a.wf32, 1.f, w[k]);
 #pragma unroll
         for (int j = 0; j < N; ++j) gw[k][j] = gb[k][j] = 0.f;
     }
-    for (long row0 = (long)blockIdx.x * per; row0 < a.rows; row0 += (long)gridDim.x * per) {
-        const long row = row0 + first;
-        const bool ok = row < a.rows;
-        float v[NV][N];
-        Pack<T> gy[NV], ds[NV];
-        float s1[1] = {0.f};
+    for (long lead = (long)blockIdx.x * per; lead < a.rows; lead += step, row += step) {
+        const bool ok = row < a.rows, more = row + step < a.rows;
+        Pack<T> xn[NV], gn[NV], ds[NV];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const long c = (long)(k * G + sub) * N;
-            const long hv = ok ? have[k] : 0;
-            const Pack<T> p = load_pack<AL>((const T*)a.x + row * a.ldx + c, hv);
-            gy[k] = load_pack<AL>((const T*)a.dy + row * a.lddy + c, hv);
-            if (a.ds) ds[k] = load_pack<AL>((const T*)a.ds + row * a.C + c, hv);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                v[k][j] = (float)p.e[j];
-                s1[0] += v[k][j];
-            }
+            if (a.ds) ds[k] = sp[k].template load<LAST>((const T*)a.ds + row * a.C, ok);
+            xn[k] = sp[k].template load<LAST>((const T*)a.x + (row + step) * a.ldx, more);
+            gn[k] = sp[k].template load<LAST>((const T*)a.dy + (row + step) * a.lddy, more);
         }
+        float s1[1] = {0.f};
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j) s1[0] += sp[k].mine(j) ? (float)x[k].e[j] : 0.f;
         row_sum(s1);
         const float m0 = s1[0] * invC;
         float m[4] = {0.f, 0.f, 0.f, 0.f};
+        float v[NV][N];
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                v[k][j] = (AL ? have[k] > 0 : j < have[k]) ? v[k][j] - m0 : 0.f;
-                const float g = (float)gy[k].e[j] * w[k][j];
-                m[0] += v[k][j];
-                m[1] += v[k][j] * v[k][j];
+                v[k][j] = (float)x[k].e[j] - m0;
+                const float t = sp[k].mine(j) ? v[k][j] : 0.f;
+                const float g = sp[k].mine(j) ? (float)gy[k].e[j] * w[k][j] : 0.f;
+                m[0] += t;
+                m[1] += t * t;
                 m[2] += g;
-                m[3] += g * v[k][j];
+                m[3] += g * t;
             }
         row_sum(m);
         const float delta = m[0] * invC;
@@ -255,8 +337,6 @@ __global__ __launch_bounds__(256) void ln_bwd_k(NormArgs a, Drop d) {
         const float c1 = m[2] * invC, c2 = (m[3] - delta * m[2]) * r * invC;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const long hv = ok ? have[k] : 0;
-            const long i = row * a.C + (long)(k * G + sub) * N;
             float g[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
@@ -273,19 +353,21 @@ __global__ __launch_bounds__(256) void ln_bwd_k(NormArgs a, Drop d) {
             if (a.dres) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) p.e[j] = (T)g[j];
-                store_pack<AL>((T*)a.dres + i, hv, p);
+                sp[k].store((T*)a.dres + row * a.C, ok, p);
             }
             if (a.dx) {
-                if (d.mode && hv > 0) {
+                if (d.mode && ok && sp[k].any()) {
                     uint32_t u[N];
-                    drop_words<N, AL>(d, sid, i, hv, u);
+                    drop_words<N, COLS == ALIGNED>(d, sid, row * a.C + sp[k].c, sp[k].hi, u);
 #pragma unroll
                     for (int j = 0; j < N; ++j) g[j] = u[j] >= d.least ? g[j] * d.scale : 0.f;
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j) p.e[j] = (T)g[j];
-                store_pack<AL>((T*)a.dx + i, hv, p);
+                sp[k].store((T*)a.dx + row * a.C, ok, p);
             }
+            x[k] = xn[k];
+            gy[k] = gn[k];
         }
     }
     if (!a.dw && !a.db) return;
@@ -293,19 +375,7 @@ __global__ __launch_bounds__(256) void ln_bwd_k(NormArgs a, Drop d) {
     for (int which = 0; which < 2; ++which) {
         float* out = a.part + ((long)blockIdx.x * 2 + which) * a.C;
         void* res = which ? a.db : a.dw;
-        if (BLK) {
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const long c = (long)(k * G + sub) * N + j;
-                    const float t = which ? gb[k][j] : gw[k][j];
-                    if (c < a.C) {
-                        if (gridDim.x > 1) out[c] = t;
-                        else if (res) put_param<T>(res, a.wf32, c, t, a.accumulate);
-                    }
-                }
-        } else {
+        if (NT == 64) {
             // rows of one wave that share columns, then the four waves
 #pragma unroll
             for (int k = 0; k < NV; ++k)
@@ -313,7 +383,8 @@ __global__ __launch_bounds__(256) void ln_bwd_k(NormArgs a, Drop d) {
                 for (int j = 0; j < N; ++j) {
                     float t = which ? gb[k][j] : gw[k][j];
                     for (int o = G; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
-                    if (lane < G) fold[((threadIdx.x >> 6) * NV + k) * 64 * N + lane * N + j] = t;
+                    if (lane < G && sp[k].mine(j))
+                        fold[((threadIdx.x >> 6) * NV + k) * 64 * N + (int)(sp[k].c - (long)k * G * N) + j] = t;
                 }
             __syncthreads();
             for (long c = threadIdx.x; c < a.C; c += 256) {
@@ -324,6 +395,17 @@ __global__ __launch_bounds__(256) void ln_bwd_k(NormArgs a, Drop d) {
                 else if (res) put_param<T>(res, a.wf32, c, t, a.accumulate);
             }
             __syncthreads();
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (sp[k].mine(j)) {
+                        const long c = sp[k].c + j;
+                        const float t = which ? gb[k][j] : gw[k][j];
+                        if (gridDim.x > 1) out[c] = t;
+                        else if (res) put_param<T>(res, a.wf32, c, t, a.accumulate);
+                    }
         }
     }
 }
@@ -352,40 +434,37 @@ __host__ __device__ static inline SplitPlan split_plan(long C, int size) {
     return s;
 }
 
-template <typename T, bool AL, bool RES, bool BWD>
+template <typename T, int COLS, bool RES, bool BWD>
 __global__ __launch_bounds__(256) void ln_split_stats_k(NormArgs a, Drop d, Chunk* __restrict__ st) {
     constexpr int N = Pack<T>::N;
-    __shared__ float sh[2][4][4];
-    RowSum<true> row_sum{sh, 6, 0};
+    __shared__ float4 sh[2][4];
+    RowSum<256> row_sum{sh, 6, 0};
     const SplitPlan sp = split_plan(a.C, sizeof(T));
     const uint64_t sid = RES ? drop_sid(d) : 0;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         double n = 0, mean = 0, m2 = 0, G = 0, H = 0;
         for (long t = blockIdx.x * sp.per; t < (blockIdx.x + 1) * sp.per && t < sp.tiles; ++t) {
-            float v[SPLIT_NV][N], g[SPLIT_NV][N];
+            Pack<T> x[SPLIT_NV];
+            float g[SPLIT_NV][N];
+            Span<T, COLS> c[SPLIT_NV];
             float s1[1] = {0.f};
 #pragma unroll
             for (int k = 0; k < SPLIT_NV; ++k) {
-                const long c = t * sp.tile + (long)(k * 256 + threadIdx.x) * N;
-                const long hv = a.C - c;
-                Pack<T> p = load_pack<AL>((const T*)a.x + row * a.ldx + c, hv);
+                c[k] = Span<T, COLS>((t * SPLIT_NV + k) * 256 + threadIdx.x, a.C);
+                x[k] = c[k].load((const T*)a.x + row * a.ldx, true);
                 if (RES) {
-                    const long i = row * a.C + c;
-                    const Pack<T> q = load_pack<AL>((const T*)a.res + i, hv);
-                    if (hv > 0) p = add_drop<T, AL>(p, q, d, sid, i, hv);
-                    store_pack<AL>((T*)a.s + i, hv, p);
+                    const Pack<T> q = c[k].load((const T*)a.res + row * a.C, true);
+                    if (c[k].any()) x[k] = add_drop<T, COLS>(x[k], q, d, sid, row * a.C + c[k].c, c[k].hi);
+                    c[k].store((T*)a.s + row * a.C, true, x[k]);
                 }
                 if (BWD) {
-                    const Pack<T> q = load_pack<AL>((const T*)a.dy + row * a.lddy + c, hv);
-                    load_params<AL, T>(a.weight, a.wf32, c, hv, 1.f, g[k]);
+                    const Pack<T> q = c[k].load((const T*)a.dy + row * a.lddy, true);
+                    c[k].params(a.weight, a.wf32, 1.f, g[k]);
 #pragma unroll
-                    for (int j = 0; j < N; ++j) g[k][j] *= (float)q.e[j];
+                    for (int j = 0; j < N; ++j) g[k][j] = c[k].mine(j) ? g[k][j] * (float)q.e[j] : 0.f;
                 }
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    v[k][j] = (AL || j < hv) ? (float)p.e[j] : 0.f;
-                    s1[0] += v[k][j];
-                }
+                for (int j = 0; j < N; ++j) s1[0] += c[k].mine(j) ? (float)x[k].e[j] : 0.f;
             }
             row_sum(s1);
             const long nt = a.C - t * sp.tile < sp.tile ? a.C - t * sp.tile : sp.tile;
@@ -395,13 +474,12 @@ __global__ __launch_bounds__(256) void ln_split_stats_k(NormArgs a, Drop d, Chun
             for (int k = 0; k < SPLIT_NV; ++k)
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    const long hv = a.C - (t * sp.tile + (long)(k * 256 + threadIdx.x) * N);
-                    const float x = (AL ? hv > 0 : j < hv) ? v[k][j] - m0 : 0.f;
-                    m[0] += x;
-                    m[1] += x * x;
+                    const float v = c[k].mine(j) ? (float)x[k].e[j] - m0 : 0.f;
+                    m[0] += v;
+                    m[1] += v * v;
                     if (BWD) {
                         m[2] += g[k][j];
-                        m[3] += g[k][j] * x;
+                        m[3] += g[k][j] * v;
                     }
                 }
             row_sum(m);
@@ -429,113 +507,152 @@ __global__ __launch_bounds__(256) void ln_split_stats_k(NormArgs a, Drop d, Chun
         }
     }
 }
-// Every wave joins all chunks of the row by itself: the same operations in the same order, no barrier.
+// Every wave joins all chunks of the row by itself: the same operations in the same order, no barrier.  Means are taken
+// relative to the first chunk's, which leaves numbers of the size of the deviations: floats hold those.
 struct RowStats {
     float hi, lo, r, c1, c2;              // mean = hi + lo
 };
 template <bool BWD>
 __device__ __forceinline__ RowStats join_chunks(const Chunk* __restrict__ st, const SplitPlan& sp, long C, float eps) {
+    constexpr int PER = SPLIT_MAX / 64;
     const int lane = threadIdx.x & 63;
     const long whole = sp.per * sp.tile;
-    double sum = 0;
-    for (long k = lane; k < sp.chunks; k += 64) sum += st[k].mean * (double)(k + 1 < sp.chunks ? whole : C - k * whole);
-    const double mean = wave_sum_d(sum) / (double)C;
-    double m2 = 0, G = 0, H = 0;
-    for (long k = lane; k < sp.chunks; k += 64) {
-        const Chunk c = st[k];
-        const double e = c.mean - mean;
-        m2 += (double)c.m2 + e * e * (double)(k + 1 < sp.chunks ? whole : C - k * whole);
-        if (BWD) {
-            G += c.g;
-            H += (double)c.h + (double)c.g * e;
-        }
+    const float invC = 1.0f / (float)C;
+    const double base = st[0].mean;
+    float e[PER], n[PER], s1[1] = {0.f};
+    Chunk c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const long k = lane + 64 * i;
+        const bool in = k < sp.chunks;
+        if (in) c[i] = st[k];
+        n[i] = in ? (float)(k + 1 < sp.chunks ? whole : C - k * whole) : 0.f;
+        e[i] = in ? (float)(c[i].mean - base) : 0.f;
+        s1[0] += n[i] * e[i];
     }
-    m2 = wave_sum_d(m2);
+    lanes_sum(s1, 6);
+    const float off = s1[0] * invC;
+    float m[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (n[i] == 0.f) continue;
+        const float x = e[i] - off;
+        m[0] += c[i].m2 + n[i] * x * x;
+        m[1] += c[i].g;
+        m[2] += c[i].h + c[i].g * x;
+    }
+    lanes_sum(m, 6);
+    const double mean = base + (double)off;
     RowStats s;
     s.hi = (float)mean;
     s.lo = (float)(mean - (double)s.hi);
-    s.r = rsqrtf((float)(m2 / (double)C) + eps);
-    if (BWD) {
-        s.c1 = (float)(wave_sum_d(G) / (double)C);
-        s.c2 = (float)(wave_sum_d(H) / (double)C) * s.r;
-    }
+    s.r = rsqrtf(m[0] * invC + eps);
+    s.c1 = BWD ? m[1] * invC : 0.f;
+    s.c2 = BWD ? m[2] * invC * s.r : 0.f;
     return s;
 }
-template <typename T, bool AL>
+template <typename T, int COLS>
 __global__ __launch_bounds__(256) void ln_split_fwd_k(NormArgs a, const Chunk* __restrict__ st) {
     constexpr int N = Pack<T>::N;
     const SplitPlan sp = split_plan(a.C, sizeof(T));
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const T* src = a.s ? (const T*)a.s + row * a.C : (const T*)a.x + row * a.ldx;
+        Span<T, COLS> c[SPLIT_NV];
+        Pack<T> x[SPLIT_NV];
+#pragma unroll
+        for (int k = 0; k < SPLIT_NV; ++k) {
+            c[k] = Span<T, COLS>((blockIdx.x * (long)SPLIT_NV + k) * 256 + threadIdx.x, a.C);
+            x[k] = c[k].load(src, true);
+        }
         const RowStats s = join_chunks<false>(st + row * sp.chunks, sp, a.C, a.eps);
 #pragma unroll
         for (int k = 0; k < SPLIT_NV; ++k) {
-            const long c = blockIdx.x * sp.tile + (long)(k * 256 + threadIdx.x) * N;
-            const long hv = a.C - c;
             float w[N], b[N];
-            load_params<AL, T>(a.weight, a.wf32, c, hv, 1.f, w);
-            load_params<AL, T>(a.bias, a.wf32, c, hv, 0.f, b);
-            const Pack<T> p = a.s ? load_pack<AL>((const T*)a.s + row * a.C + c, hv)
-                                  : load_pack<AL>((const T*)a.x + row * a.ldx + c, hv);
+            c[k].params(a.weight, a.wf32, 1.f, w);
+            c[k].params(a.bias, a.wf32, 0.f, b);
             Pack<T> o;
 #pragma unroll
-            for (int j = 0; j < N; ++j) o.e[j] = (T)((((float)p.e[j] - s.hi) - s.lo) * s.r * w[j] + b[j]);
-            store_pack<AL>((T*)a.y + row * a.C + c, hv, o);
+            for (int j = 0; j < N; ++j) o.e[j] = (T)((((float)x[k].e[j] - s.hi) - s.lo) * s.r * w[j] + b[j]);
+            c[k].store((T*)a.y + row * a.C, true, o);
         }
     }
 }
-// Backward: block (tile, part of the rows) keeps the parameter gradients of its columns in registers.
-template <typename T, bool AL>
+// Backward: block (tile, part of the rows) keeps the parameter gradients of its columns in registers.  Its waves first
+// join the chunks of a batch of rows, four rows at a time, so that the rows behind are one stream of loads.
+constexpr int SPLIT_BATCH = 16;
+template <typename T, int COLS>
 __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const Chunk* __restrict__ st) {
     constexpr int N = Pack<T>::N;
+    __shared__ RowStats stats[SPLIT_BATCH];
     const SplitPlan sp = split_plan(a.C, sizeof(T));
     const uint64_t sid = drop_sid(d);
+    const int wave = threadIdx.x >> 6;
     float w[SPLIT_NV][N], gw[SPLIT_NV][N], gb[SPLIT_NV][N];
+    Span<T, COLS> c[SPLIT_NV];
+    Pack<T> x[SPLIT_NV], gy[SPLIT_NV];
+    long row = blockIdx.y;
 #pragma unroll
     for (int k = 0; k < SPLIT_NV; ++k) {
-        const long c = blockIdx.x * sp.tile + (long)(k * 256 + threadIdx.x) * N;
-        load_params<AL, T>(a.weight, a.wf32, c, a.C - c, 1.f, w[k]);
+        c[k] = Span<T, COLS>((blockIdx.x * (long)SPLIT_NV + k) * 256 + threadIdx.x, a.C);
+        x[k] = c[k].load((const T*)a.x + row * a.ldx, row < a.rows);
+        gy[k] = c[k].load((const T*)a.dy + row * a.lddy, row < a.rows);
+        c[k].params(a.weight, a.wf32, 1.f, w[k]);
 #pragma unroll
         for (int j = 0; j < N; ++j) gw[k][j] = gb[k][j] = 0.f;
     }
-    for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        const RowStats s = join_chunks<true>(st + row * sp.chunks, sp, a.C, a.eps);
+    for (int at = 0; row < a.rows; row += gridDim.y, at = (at + 1) % SPLIT_BATCH) {
+        if (at == 0) {
+            __syncthreads();                                     // the last batch has been read
+            for (int i = wave; i < SPLIT_BATCH; i += 4) {
+                const long r = row + (long)i * gridDim.y;
+                if (r >= a.rows) break;
+                const RowStats s = join_chunks<true>(st + r * sp.chunks, sp, a.C, a.eps);
+                if ((threadIdx.x & 63) == 0) stats[i] = s;
+            }
+            __syncthreads();
+        }
+        const RowStats s = stats[at];
+        const long next = row + gridDim.y;
+        Pack<T> xn[SPLIT_NV], gn[SPLIT_NV], ds[SPLIT_NV];
 #pragma unroll
         for (int k = 0; k < SPLIT_NV; ++k) {
-            const long c = blockIdx.x * sp.tile + (long)(k * 256 + threadIdx.x) * N;
-            const long hv = a.C - c, i = row * a.C + c;
-            const Pack<T> p = load_pack<AL>((const T*)a.x + row * a.ldx + c, hv);
-            const Pack<T> q = load_pack<AL>((const T*)a.dy + row * a.lddy + c, hv);
+            if (a.ds) ds[k] = c[k].load((const T*)a.ds + row * a.C, true);
+            xn[k] = c[k].load((const T*)a.x + next * a.ldx, next < a.rows);
+            gn[k] = c[k].load((const T*)a.dy + next * a.lddy, next < a.rows);
+        }
+#pragma unroll
+        for (int k = 0; k < SPLIT_NV; ++k) {
             float g[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float dy = (float)q.e[j];
-                const float h = (((float)p.e[j] - s.hi) - s.lo) * s.r;
+                const float dy = (float)gy[k].e[j];
+                const float h = (((float)x[k].e[j] - s.hi) - s.lo) * s.r;
                 gw[k][j] += dy * h;
                 gb[k][j] += dy;
                 g[j] = s.r * (dy * w[k][j] - s.c1 - h * s.c2);
             }
-            if (a.ds) {
-                const Pack<T> e = load_pack<AL>((const T*)a.ds + i, hv);
+            if (a.ds)
 #pragma unroll
-                for (int j = 0; j < N; ++j) g[j] += (float)e.e[j];
-            }
+                for (int j = 0; j < N; ++j) g[j] += (float)ds[k].e[j];
             Pack<T> o;
             if (a.dres) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) o.e[j] = (T)g[j];
-                store_pack<AL>((T*)a.dres + i, hv, o);
+                c[k].store((T*)a.dres + row * a.C, true, o);
             }
             if (a.dx) {
-                if (d.mode && hv > 0) {
+                if (d.mode && c[k].any()) {
                     uint32_t u[N];
-                    drop_words<N, AL>(d, sid, i, hv, u);
+                    drop_words<N, COLS == ALIGNED>(d, sid, row * a.C + c[k].c, c[k].hi, u);
 #pragma unroll
                     for (int j = 0; j < N; ++j) g[j] = u[j] >= d.least ? g[j] * d.scale : 0.f;
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j) o.e[j] = (T)g[j];
-                store_pack<AL>((T*)a.dx + i, hv, o);
+                c[k].store((T*)a.dx + row * a.C, true, o);
             }
+            x[k] = xn[k];
+            gy[k] = gn[k];
         }
     }
     if (!a.dw && !a.db) return;
@@ -543,29 +660,34 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
     for (int k = 0; k < SPLIT_NV; ++k)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const long c = blockIdx.x * sp.tile + (long)(k * 256 + threadIdx.x) * N + j;
-            if (c >= a.C) continue;
+            if (!c[k].mine(j)) continue;
+            const long i = c[k].c + j;
             if (gridDim.y > 1) {
-                a.part[((long)blockIdx.y * 2 + 0) * a.C + c] = gw[k][j];
-                a.part[((long)blockIdx.y * 2 + 1) * a.C + c] = gb[k][j];
+                a.part[((long)blockIdx.y * 2 + 0) * a.C + i] = gw[k][j];
+                a.part[((long)blockIdx.y * 2 + 1) * a.C + i] = gb[k][j];
             } else {
-                if (a.dw) put_param<T>(a.dw, a.wf32, c, gw[k][j], a.accumulate);
-                if (a.db) put_param<T>(a.db, a.wf32, c, gb[k][j], a.accumulate);
+                if (a.dw) put_param<T>(a.dw, a.wf32, i, gw[k][j], a.accumulate);
+                if (a.db) put_param<T>(a.db, a.wf32, i, gb[k][j], a.accumulate);
             }
         }
 }
 
-// the blocks' partial sums joined: 16 columns to a block, 64 threads down each, in a fixed order
-template <typename T>
+// the blocks' partial sums joined: 1024 / DOWN columns to a block, DOWN threads down each, in a fixed order
+template <typename T, int DOWN>
 __global__ __launch_bounds__(1024) void ln_param_sum_k(const float* __restrict__ part, long parts, NormArgs a) {
-    __shared__ float sh[64][17];
-    const int col = threadIdx.x & 15, down = threadIdx.x >> 4;
-    const long i = (long)blockIdx.x * 16 + col, C2 = 2 * a.C;
+    constexpr int ACROSS = 1024 / DOWN;
+    __shared__ float sh[DOWN][ACROSS + 1];
+    const int col = threadIdx.x % ACROSS, down = threadIdx.x / ACROSS;
+    const long i = (long)blockIdx.x * ACROSS + col, C2 = 2 * a.C;
     float t = 0.f;
-    if (i < C2)
-        for (long k = down; k < parts; k += 64) t += part[k * C2 + i];
+    if (i < C2) {
+        long k = down;
+        for (; k + 3 * DOWN < parts; k += 4 * DOWN)          // four loads at a time
+            t += (part[k * C2 + i] + part[(k + DOWN) * C2 + i]) + (part[(k + 2 * DOWN) * C2 + i] + part[(k + 3 * DOWN) * C2 + i]);
+        for (; k < parts; k += DOWN) t += part[k * C2 + i];
+    }
     sh[down][col] = t;
-    for (int o = 32; o > 0; o >>= 1) {
+    for (int o = DOWN / 2; o > 0; o >>= 1) {
         __syncthreads();
         if (down < o) sh[down][col] += sh[down + o][col];
     }
@@ -575,25 +697,37 @@ __global__ __launch_bounds__(1024) void ln_param_sum_k(const float* __restrict__
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
-// Which kernel: a function of the row length and the type alone, so that a row's result does not depend on what is
-// computed beside it.
-enum Form { WAVE1, WAVE2, BLOCK1, BLOCK2, BLOCK4, SPLIT };
-static Form ln_form(long C, int type, int* lg) {
-    const long n = 16 / type_size(type), packs = cdiv(C, n);
-    *lg = 0;
+// Which kernel: a function of the row length, the type and the direction alone, so that a row's result does not depend
+// on what is computed beside it.
+struct Form {
+    int nt, nv, lg;         // nt 0: split
+};
+static Form ln_form(long C, int type, bool bwd) {
+    const long packs = cdiv(C, 16 / type_size(type));
     if (packs <= 64) {
-        while ((1L << *lg) < packs) ++*lg;
-        return WAVE1;
+        int lg = 0;
+        while ((1L << lg) < packs) ++lg;
+        return {64, 1, lg};
     }
-    *lg = 6;
-    return packs <= 128 ? WAVE2 : packs <= 256 ? BLOCK1 : packs <= 512 ? BLOCK2 : packs <= 1024 ? BLOCK4 : SPLIT;
+    if (packs <= 128) return bwd ? Form{128, 1, 6} : Form{64, 2, 6};
+    if (packs <= 256) return {256, 1, 6};
+    if (packs <= 512) return {512, 1, 6};
+    if (packs <= 1024) return {1024, 1, 6};
+    if (packs <= 2048 && (!bwd || type == SIV_F32)) return {1024, 2, 6};
+    return {0, 0, 0};
 }
-static long ln_blocks(long rows, Form f, int lg, bool bwd) {
-    const long per = f <= WAVE2 ? 256 >> lg : 1;
+static long ln_blocks(long rows, const Form& f, bool bwd) {
+    const long per = f.nt == 64 ? 256 >> f.lg : 1;
     const long steps = cdiv(rows, per);
-    const long cap = bwd ? 1024 : 2048;
-    if (bwd && steps <= 2) return 1;                 // the parameters' gradients in one launch
-    return steps < cap ? steps : cap;
+    const int threads = f.nt == 64 ? 256 : f.nt;
+    if (!bwd) {
+        const long cap = f.nt > 64 ? 2048 * 256L / threads : f.nv == 2 ? 8192 : 1L << 20;
+        return steps < cap ? steps : cap;
+    }
+    if (steps <= 4) return 1;                        // the parameters' gradients in one launch
+    const long cap = f.nt == 64 ? 768 : 1024 * 256L / threads;
+    const long b = steps / 4 > 256 ? steps / 4 : 256;
+    return std::min(std::min(b, cap), steps);
 }
 // parts of the rows in the second launch of the split form: enough blocks for the chip, eight rows each at least
 static long ln_split_parts(long rows, const SplitPlan& sp) {
@@ -602,14 +736,13 @@ static long ln_split_parts(long rows, const SplitPlan& sp) {
     return p < 1 ? 1 : p;
 }
 static size_t ln_ws_bytes(long rows, long C, int type, int bwd) {
-    int lg;
-    const Form f = ln_form(C, type, &lg);
-    if (f == SPLIT) {
+    const Form f = ln_form(C, type, bwd);
+    if (f.nt == 0) {
         const SplitPlan sp = split_plan(C, type_size(type));
         const long parts = bwd ? ln_split_parts(rows, sp) : 1;
         return align256((size_t)rows * sp.chunks * sizeof(Chunk)) + (parts > 1 ? (size_t)parts * 2 * C * 4 : 0);
     }
-    const long blocks = bwd ? ln_blocks(rows, f, lg, true) : 1;
+    const long blocks = bwd ? ln_blocks(rows, f, true) : 1;
     return blocks > 1 ? (size_t)blocks * 2 * C * 4 : 0;
 }
 static int ln_check(const char* what, const NormArgs& a, int type, int wtype) {
@@ -626,93 +759,103 @@ static int ln_check_ws(const char* what, size_t need, const void* ws, size_t hav
     SIV_CHECK_ARG(need == 0 || ((uintptr_t)ws & 15) == 0, "%s: the workspace must be 16-byte aligned", what);
     return SIV_OK;
 }
-static bool ln_aligned(const NormArgs& a, int type) {
+static Cols ln_cols(const NormArgs& a, int type) {
     const long n = 16 / type_size(type);
+    if (a.C < n) return SHORT;
     return a.C % n == 0 && a.ldx % n == 0 && a.lddy % n == 0 && aligned16(a.x) && aligned16(a.res) && aligned16(a.dy) &&
-           aligned16(a.ds) && aligned16(a.s) && aligned16(a.y) && aligned16(a.dx) && aligned16(a.dres);
+                   aligned16(a.ds) && aligned16(a.s) && aligned16(a.y) && aligned16(a.dx) && aligned16(a.dres)
+               ? ALIGNED
+               : OVERLAP;
 }
-
-template <typename T, bool AL, bool RES>
-static void ln_fwd_launch(const NormArgs& a, const Drop& d, Form f, unsigned g, hipStream_t st) {
-    switch (f) {
-        case WAVE1: ln_fwd_k<T, 1, false, AL, RES><<<g, 256, 0, st>>>(a, d); break;
-        case WAVE2: ln_fwd_k<T, 2, false, AL, RES><<<g, 256, 0, st>>>(a, d); break;
-        case BLOCK1: ln_fwd_k<T, 1, true, AL, RES><<<g, 256, 0, st>>>(a, d); break;
-        case BLOCK2: ln_fwd_k<T, 2, true, AL, RES><<<g, 256, 0, st>>>(a, d); break;
-        default: ln_fwd_k<T, 4, true, AL, RES><<<g, 256, 0, st>>>(a, d); break;
+// calls f with std::integral_constant of the column kind
+template <typename F>
+static int with_cols(Cols c, F f) {
+    if (c == ALIGNED) return f(std::integral_constant<int, ALIGNED>());
+    if (c == OVERLAP) return f(std::integral_constant<int, OVERLAP>());
+    return f(std::integral_constant<int, SHORT>());
+}
+template <typename T, int COLS, bool RES>
+static void ln_fwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
+    if (f.nt == 64 && f.nv == 1) ln_fwd_k<T, 1, 64, COLS, RES><<<g, 256, 0, st>>>(a, d);
+    else if constexpr (COLS != SHORT) {              // a row of less than a pack is one lane's
+        if (f.nt == 64) ln_fwd_k<T, 2, 64, COLS, RES><<<g, 256, 0, st>>>(a, d);
+        else if (f.nt == 256) ln_fwd_k<T, 1, 256, COLS, RES><<<g, 256, 0, st>>>(a, d);
+        else if (f.nt == 512) ln_fwd_k<T, 1, 512, COLS, RES><<<g, 512, 0, st>>>(a, d);
+        else if (f.nv == 1) ln_fwd_k<T, 1, 1024, COLS, RES><<<g, 1024, 0, st>>>(a, d);
+        else ln_fwd_k<T, 2, 1024, COLS, RES><<<g, 1024, 0, st>>>(a, d);
     }
 }
-template <typename T, bool AL>
-static void ln_bwd_launch(const NormArgs& a, const Drop& d, Form f, unsigned g, hipStream_t st) {
-    switch (f) {
-        case WAVE1: ln_bwd_k<T, 1, false, AL><<<g, 256, 0, st>>>(a, d); break;
-        case WAVE2: ln_bwd_k<T, 2, false, AL><<<g, 256, 0, st>>>(a, d); break;
-        case BLOCK1: ln_bwd_k<T, 1, true, AL><<<g, 256, 0, st>>>(a, d); break;
-        case BLOCK2: ln_bwd_k<T, 2, true, AL><<<g, 256, 0, st>>>(a, d); break;
-        default: ln_bwd_k<T, 4, true, AL><<<g, 256, 0, st>>>(a, d); break;
+template <typename T, int COLS>
+static void ln_bwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
+    if (f.nt == 64 && f.nv == 1) ln_bwd_k<T, 1, 64, COLS><<<g, 256, 0, st>>>(a, d);
+    else if constexpr (COLS != SHORT) {
+        if (f.nt == 128) ln_bwd_k<T, 1, 128, COLS><<<g, 128, 0, st>>>(a, d);
+        else if (f.nt == 256) ln_bwd_k<T, 1, 256, COLS><<<g, 256, 0, st>>>(a, d);
+        else if (f.nt == 512) ln_bwd_k<T, 1, 512, COLS><<<g, 512, 0, st>>>(a, d);
+        else if (f.nv == 1) ln_bwd_k<T, 1, 1024, COLS><<<g, 1024, 0, st>>>(a, d);
+        else if constexpr (sizeof(T) == 4) ln_bwd_k<T, 2, 1024, COLS><<<g, 1024, 0, st>>>(a, d);
     }
 }
 static unsigned grid_y(long n) { return (unsigned)(n < 65535 ? n : 65535); }
 
 static int ln_fwd(const char* what, NormArgs a, const Drop& d, bool res, int type, void* ws, size_t ws_bytes, hipStream_t st) {
     if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, type, 0), ws, ws_bytes)) return rc;
-    const Form f = ln_form(a.C, type, &a.lg);
-    const bool al = ln_aligned(a, type);
-    const unsigned g = (unsigned)ln_blocks(a.rows, f, a.lg, false);
+    const Form f = ln_form(a.C, type, false);
+    a.lg = f.lg;
     return with_type(type, [&](auto* t) {
         typedef typename std::remove_reference<decltype(*t)>::type T;
-        if (f != SPLIT) {
-            if (al && res) ln_fwd_launch<T, true, true>(a, d, f, g, st);
-            else if (al) ln_fwd_launch<T, true, false>(a, d, f, g, st);
-            else if (res) ln_fwd_launch<T, false, true>(a, d, f, g, st);
-            else ln_fwd_launch<T, false, false>(a, d, f, g, st);
+        return with_cols(ln_cols(a, type), [&](auto kind) {
+            constexpr int COLS = decltype(kind)::value;
+            if (f.nt) {
+                const unsigned g = (unsigned)ln_blocks(a.rows, f, false);
+                if (res) ln_fwd_launch<T, COLS, true>(a, d, f, g, st);
+                else ln_fwd_launch<T, COLS, false>(a, d, f, g, st);
+            } else if constexpr (COLS != SHORT) {
+                const SplitPlan sp = split_plan(a.C, sizeof(T));
+                const dim3 gs((unsigned)sp.chunks, grid_y(a.rows)), ga((unsigned)sp.tiles, grid_y(a.rows));
+                Chunk* c = (Chunk*)ws;
+                if (res) ln_split_stats_k<T, COLS, true, false><<<gs, 256, 0, st>>>(a, d, c);
+                else ln_split_stats_k<T, COLS, false, false><<<gs, 256, 0, st>>>(a, d, c);
+                SIV_CHECK_LAUNCH(what);
+                ln_split_fwd_k<T, COLS><<<ga, 256, 0, st>>>(a, c);
+            }
             SIV_CHECK_LAUNCH(what);
             return SIV_OK;
-        }
-        const SplitPlan sp = split_plan(a.C, sizeof(T));
-        const dim3 gs((unsigned)sp.chunks, grid_y(a.rows)), ga((unsigned)sp.tiles, grid_y(a.rows));
-        Chunk* c = (Chunk*)ws;
-        if (al && res) ln_split_stats_k<T, true, true, false><<<gs, 256, 0, st>>>(a, d, c);
-        else if (al) ln_split_stats_k<T, true, false, false><<<gs, 256, 0, st>>>(a, d, c);
-        else if (res) ln_split_stats_k<T, false, true, false><<<gs, 256, 0, st>>>(a, d, c);
-        else ln_split_stats_k<T, false, false, false><<<gs, 256, 0, st>>>(a, d, c);
-        SIV_CHECK_LAUNCH(what);
-        if (al) ln_split_fwd_k<T, true><<<ga, 256, 0, st>>>(a, c);
-        else ln_split_fwd_k<T, false><<<ga, 256, 0, st>>>(a, c);
-        SIV_CHECK_LAUNCH(what);
-        return SIV_OK;
+        });
     });
 }
 static int ln_bwd(const char* what, NormArgs a, const Drop& d, int type, void* ws, size_t ws_bytes, hipStream_t st) {
     if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, type, 1), ws, ws_bytes)) return rc;
-    const Form f = ln_form(a.C, type, &a.lg);
-    const bool al = ln_aligned(a, type);
+    const Form f = ln_form(a.C, type, true);
+    a.lg = f.lg;
     return with_type(type, [&](auto* t) {
         typedef typename std::remove_reference<decltype(*t)>::type T;
-        long parts;
-        if (f != SPLIT) {
-            parts = ln_blocks(a.rows, f, a.lg, true);
-            a.part = (float*)ws;
-            if (al) ln_bwd_launch<T, true>(a, d, f, (unsigned)parts, st);
-            else ln_bwd_launch<T, false>(a, d, f, (unsigned)parts, st);
-        } else {
-            const SplitPlan sp = split_plan(a.C, sizeof(T));
-            Chunk* c = (Chunk*)ws;
-            a.part = (float*)((char*)ws + align256((size_t)a.rows * sp.chunks * sizeof(Chunk)));
-            parts = ln_split_parts(a.rows, sp);
-            const dim3 gs((unsigned)sp.chunks, grid_y(a.rows)), ga((unsigned)sp.tiles, (unsigned)parts);
-            if (al) ln_split_stats_k<T, true, false, true><<<gs, 256, 0, st>>>(a, d, c);
-            else ln_split_stats_k<T, false, false, true><<<gs, 256, 0, st>>>(a, d, c);
+        return with_cols(ln_cols(a, type), [&](auto kind) {
+            constexpr int COLS = decltype(kind)::value;
+            long parts = 1;
+            if (f.nt) {
+                parts = ln_blocks(a.rows, f, true);
+                a.part = (float*)ws;
+                ln_bwd_launch<T, COLS>(a, d, f, (unsigned)parts, st);
+            } else if constexpr (COLS != SHORT) {
+                const SplitPlan sp = split_plan(a.C, sizeof(T));
+                Chunk* c = (Chunk*)ws;
+                a.part = (float*)((char*)ws + align256((size_t)a.rows * sp.chunks * sizeof(Chunk)));
+                parts = ln_split_parts(a.rows, sp);
+                const dim3 gs((unsigned)sp.chunks, grid_y(a.rows)), ga((unsigned)sp.tiles, (unsigned)parts);
+                ln_split_stats_k<T, COLS, false, true><<<gs, 256, 0, st>>>(a, d, c);
+                SIV_CHECK_LAUNCH(what);
+                ln_split_bwd_k<T, COLS><<<ga, 256, 0, st>>>(a, d, c);
+            }
             SIV_CHECK_LAUNCH(what);
-            if (al) ln_split_bwd_k<T, true><<<ga, 256, 0, st>>>(a, d, c);
-            else ln_split_bwd_k<T, false><<<ga, 256, 0, st>>>(a, d, c);
-        }
-        SIV_CHECK_LAUNCH(what);
-        if ((a.dw || a.db) && parts > 1) {
-            ln_param_sum_k<T><<<(unsigned)cdiv(2 * a.C, 16), 1024, 0, st>>>(a.part, parts, a);
-            SIV_CHECK_LAUNCH(what);
-        }
-        return SIV_OK;
+            if ((a.dw || a.db) && parts > 1) {
+                if (parts <= 32) ln_param_sum_k<T, 4><<<(unsigned)cdiv(2 * a.C, 256), 1024, 0, st>>>(a.part, parts, a);
+                else if (parts <= 256 || a.C >= 4096) ln_param_sum_k<T, 16><<<(unsigned)cdiv(2 * a.C, 64), 1024, 0, st>>>(a.part, parts, a);
+                else ln_param_sum_k<T, 64><<<(unsigned)cdiv(2 * a.C, 16), 1024, 0, st>>>(a.part, parts, a);
+                SIV_CHECK_LAUNCH(what);
+            }
+            return SIV_OK;
+        });
     });
 }
 
