@@ -94,56 +94,66 @@ struct RowSum {
 // that it ends with the row, the columns it shares with the pack before it count there only (both store the same
 // value).  Every access is one 16-byte instruction either way.  SHORT: rows of less than a pack, element by element.
 enum Cols { SHORT, OVERLAP, ALIGNED };
+// Lanes without a column or a row are not branched around: a conditional store in a loop makes the compiler wait for
+// every store of a step before it uses what was loaded a step ahead.  They go to an offset that the buffer descriptor
+// turns away (loads give zero, stores nothing).
+constexpr uint32_t NOWHERE = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
+}
 template <typename T, int COLS>
 struct Span {
     static constexpr int N = Pack<T>::N;
-    long c;                 // first column accessed
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    uint32_t c;             // first column accessed
     int lo, hi;             // elements lo .. hi-1 of the pack are this lane's
     __device__ __forceinline__ Span() {}
-    template <int OTHER>
-    __device__ __forceinline__ explicit Span(const Span<T, OTHER>& o) : c(o.c), lo(o.lo), hi(o.hi) {}
     __device__ __forceinline__ Span(long pack, long C) {
-        c = pack * N;
-        const long have = C - c;
+        const long have = C - pack * N;
         lo = 0;
         hi = have >= N ? N : have > 0 ? (int)have : 0;
+        c = (uint32_t)(pack * N);
         if (COLS == OVERLAP && have < N) {
             lo = have > 0 ? N - (int)have : N;
             hi = N;
-            c = C - N;
+            c = (uint32_t)(C - N);
         }
     }
     __device__ __forceinline__ bool any() const { return lo < hi; }
     __device__ __forceinline__ bool mine(int j) const {
         return COLS == ALIGNED ? hi > 0 : COLS == OVERLAP ? j >= lo : j < hi;
     }
-    // does the access touch element j (a column of the row)
-    __device__ __forceinline__ bool touches(int j) const { return COLS == SHORT ? j < hi : any(); }
-    // LAST: nothing is expected to read the tensor again soon
+    // byte offset of the pack in a tensor whose rows are ld apart, from `row` rows behind the base (and `from` columns
+    // into it) on
+    __device__ __forceinline__ uint32_t at(long row, long ld, uint32_t from = 0) const {
+        return any() ? (uint32_t)((row * ld + c - from) * (long)sizeof(T)) : NOWHERE;
+    }
+    // base: the same for the whole wave.  LAST: nothing is expected to read the tensor again soon.
     template <bool LAST = false>
-    __device__ __forceinline__ Pack<T> load(const void* row, bool ok) const {
+    __device__ __forceinline__ Pack<T> load(const void* base, uint32_t off) const {
         Pack<T> v;
+        if (COLS == SHORT) {
+            const T* p = (const T*)((const char*)base + off);
 #pragma unroll
-        for (int j = 0; j < N; ++j) v.e[j] = (T)0.f;
-        if (!ok || !any()) return v;
-        const T* p = (const T*)row + c;
-        if (COLS == ALIGNED) v = LAST ? load_stream(p) : *reinterpret_cast<const Pack<T>*>(p);
-        else if (COLS == OVERLAP) __builtin_memcpy(v.e, p, 16);
-        else
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < hi) v.e[j] = p[j];
+            for (int j = 0; j < N; ++j) v.e[j] = off != NOWHERE && j < hi ? p[j] : (T)0.f;
+        } else {
+            const words w = __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(base), off, 0, LAST && COLS == ALIGNED ? 2 : 0);
+            __builtin_memcpy(v.e, &w, 16);
+        }
         return v;
     }
-    __device__ __forceinline__ void store(void* row, bool ok, const Pack<T>& v) const {
-        if (!ok || !any()) return;
-        T* p = (T*)row + c;
-        if (COLS == ALIGNED) store_stream(p, v);
-        else if (COLS == OVERLAP) __builtin_memcpy(p, v.e, 16);
-        else
+    __device__ __forceinline__ void store(void* base, uint32_t off, const Pack<T>& v) const {
+        if (COLS == SHORT) {
+            T* p = (T*)((char*)base + off);
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (j < hi) p[j] = v.e[j];
+                if (off != NOWHERE && j < hi) p[j] = v.e[j];
+        } else {
+            words w;
+            __builtin_memcpy(&w, v.e, 16);
+            // whole lines go out non-temporally: the L2, which a kernel's end writes back anyway, is left to the operands
+            __builtin_amdgcn_raw_buffer_store_b128(w, rows_rsrc(base), off, 0, COLS == ALIGNED ? 2 : 0);
+        }
     }
     // this pack's columns of a parameter vector, in as few loads as the type allows
     __device__ __forceinline__ void params(const void* w, int f32, float dflt, float (&out)[N]) const {
@@ -160,7 +170,14 @@ struct Span {
                 __builtin_memcpy(out, p, 4 * N);
             }
         } else {
-            const Pack<T> v = Span<T, COLS == SHORT ? SHORT : OVERLAP>(*this).load(w, true);
+            const T* p = (const T*)w + c;
+            Pack<T> v;
+            if (COLS == SHORT) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) v.e[j] = j < hi ? p[j] : (T)0.f;
+            } else {
+                __builtin_memcpy(v.e, p, 16);
+            }
 #pragma unroll
             for (int j = 0; j < N; ++j)
                 if (COLS != SHORT || j < hi) out[j] = (float)v.e[j];
@@ -208,35 +225,39 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_fwd_k(NormArgs a, Drop
     const long step = (long)gridDim.x * per;
     const uint64_t sid = RES ? drop_sid(d) : 0;
     const float invC = 1.0f / (float)a.C;
+    const int rin = NT == 64 ? threadIdx.x >> a.lg : 0;               // this lane's row within the step
     Span<T, COLS> sp[NV];
     float w[NV][N], b[NV][N];
-    long row = (long)blockIdx.x * per + (NT == 64 ? threadIdx.x >> a.lg : 0);
+    uint32_t ox[NV], od[NV];                                          // offsets in x, and in the dense tensors
+    long lead = (long)blockIdx.x * per;                               // first row of the step
+    bool ok = rin < a.rows - lead;
     Pack<T> x[NV], q[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         sp[k] = Span<T, COLS>(k * G + sub, a.C);
-        x[k] = sp[k].load((const T*)a.x + row * a.ldx, row < a.rows);
-        if (RES) q[k] = sp[k].load((const T*)a.res + row * a.C, row < a.rows);
+        ox[k] = sp[k].at(rin, a.ldx);
+        od[k] = sp[k].at(rin, a.C);
+        x[k] = sp[k].load((const T*)a.x + lead * a.ldx, ok ? ox[k] : NOWHERE);
+        if (RES) q[k] = sp[k].load((const T*)a.res + lead * a.C, ok ? od[k] : NOWHERE);
         sp[k].params(a.weight, a.wf32, 1.f, w[k]);
         sp[k].params(a.bias, a.wf32, 0.f, b[k]);
     }
-    // (the block's first row decides: every lane of a block makes the same number of steps)
-    for (long lead = (long)blockIdx.x * per; lead < a.rows; lead += step, row += step) {
-        const bool ok = row < a.rows, more = row + step < a.rows;
+    for (; lead < a.rows; lead += step) {
+        const bool more = rin < a.rows - (lead + step);
         Pack<T> xn[NV], qn[NV];
         if (AHEAD)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                xn[k] = sp[k].load((const T*)a.x + (row + step) * a.ldx, more);
-                if (RES) qn[k] = sp[k].load((const T*)a.res + (row + step) * a.C, more);
+                xn[k] = sp[k].load((const T*)a.x + (lead + step) * a.ldx, more ? ox[k] : NOWHERE);
+                if (RES) qn[k] = sp[k].load((const T*)a.res + (lead + step) * a.C, more ? od[k] : NOWHERE);
             }
         float v[NV][N];
         float s1[1] = {0.f};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (RES) {
-                if (ok && sp[k].any()) x[k] = add_drop<T, COLS>(x[k], q[k], d, sid, row * a.C + sp[k].c, sp[k].hi);
-                sp[k].store((T*)a.s + row * a.C, ok, x[k]);
+                x[k] = add_drop<T, COLS>(x[k], q[k], d, sid, (lead + rin) * a.C + sp[k].c, ok ? sp[k].hi : 0);
+                sp[k].store((T*)a.s + lead * a.C, ok ? od[k] : NOWHERE, x[k]);
             }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
@@ -264,10 +285,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_fwd_k(NormArgs a, Drop
             Pack<T> p;
 #pragma unroll
             for (int j = 0; j < N; ++j) p.e[j] = (T)((v[k][j] - delta) * r * w[k][j] + b[k][j]);
-            sp[k].store((T*)a.y + row * a.C, ok, p);
-            x[k] = AHEAD ? xn[k] : sp[k].load((const T*)a.x + (row + step) * a.ldx, more);
-            if (RES) q[k] = AHEAD ? qn[k] : sp[k].load((const T*)a.res + (row + step) * a.C, more);
+            sp[k].store((T*)a.y + lead * a.C, ok ? od[k] : NOWHERE, p);
+            x[k] = AHEAD ? xn[k] : sp[k].load((const T*)a.x + (lead + step) * a.ldx, more ? ox[k] : NOWHERE);
+            if (RES) q[k] = AHEAD ? qn[k] : sp[k].load((const T*)a.res + (lead + step) * a.C, more ? od[k] : NOWHERE);
         }
+        ok = more;
     }
 }
 
@@ -287,27 +309,33 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_bwd_k(NormArgs a, Drop
     const long step = (long)gridDim.x * per;
     const uint64_t sid = drop_sid(d);
     const float invC = 1.0f / (float)a.C;
+    const int rin = NT == 64 ? threadIdx.x >> a.lg : 0;
     Span<T, COLS> sp[NV];
     float w[NV][N], gw[NV][N], gb[NV][N];
-    long row = (long)blockIdx.x * per + (NT == 64 ? threadIdx.x >> a.lg : 0);
+    uint32_t ox[NV], oy[NV], od[NV];
+    long lead = (long)blockIdx.x * per;
+    bool ok = rin < a.rows - lead;
     Pack<T> x[NV], gy[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         sp[k] = Span<T, COLS>(k * G + sub, a.C);
-        x[k] = sp[k].template load<LAST>((const T*)a.x + row * a.ldx, row < a.rows);
-        gy[k] = sp[k].template load<LAST>((const T*)a.dy + row * a.lddy, row < a.rows);
+        ox[k] = sp[k].at(rin, a.ldx);
+        oy[k] = sp[k].at(rin, a.lddy);
+        od[k] = sp[k].at(rin, a.C);
+        x[k] = sp[k].template load<LAST>((const T*)a.x + lead * a.ldx, ok ? ox[k] : NOWHERE);
+        gy[k] = sp[k].template load<LAST>((const T*)a.dy + lead * a.lddy, ok ? oy[k] : NOWHERE);
         sp[k].params(a.weight, a.wf32, 1.f, w[k]);
 #pragma unroll
         for (int j = 0; j < N; ++j) gw[k][j] = gb[k][j] = 0.f;
     }
-    for (long lead = (long)blockIdx.x * per; lead < a.rows; lead += step, row += step) {
-        const bool ok = row < a.rows, more = row + step < a.rows;
+    for (; lead < a.rows; lead += step) {
+        const bool more = rin < a.rows - (lead + step);
         Pack<T> xn[NV], gn[NV], ds[NV];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (a.ds) ds[k] = sp[k].template load<LAST>((const T*)a.ds + row * a.C, ok);
-            xn[k] = sp[k].template load<LAST>((const T*)a.x + (row + step) * a.ldx, more);
-            gn[k] = sp[k].template load<LAST>((const T*)a.dy + (row + step) * a.lddy, more);
+            ds[k] = sp[k].template load<LAST>((const T*)a.ds + lead * a.C, ok && a.ds ? od[k] : NOWHERE);
+            xn[k] = sp[k].template load<LAST>((const T*)a.x + (lead + step) * a.ldx, more ? ox[k] : NOWHERE);
+            gn[k] = sp[k].template load<LAST>((const T*)a.dy + (lead + step) * a.lddy, more ? oy[k] : NOWHERE);
         }
         float s1[1] = {0.f};
 #pragma unroll
@@ -344,31 +372,23 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_bwd_k(NormArgs a, Drop
                 const float h = (v[k][j] - delta) * r;
                 gw[k][j] += dy * h;
                 gb[k][j] += dy;
-                g[j] = r * (dy * w[k][j] - c1 - h * c2);
+                g[j] = r * (dy * w[k][j] - c1 - h * c2) + (float)ds[k].e[j];
             }
-            if (a.ds)
-#pragma unroll
-                for (int j = 0; j < N; ++j) g[j] += (float)ds[k].e[j];
             Pack<T> p;
-            if (a.dres) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) p.e[j] = (T)g[j];
-                sp[k].store((T*)a.dres + row * a.C, ok, p);
+            for (int j = 0; j < N; ++j) p.e[j] = (T)g[j];
+            sp[k].store((T*)a.dres + lead * a.C, ok && a.dres ? od[k] : NOWHERE, p);
+            if (d.mode) {
+                uint32_t u[N];
+                drop_words<N, COLS == ALIGNED>(d, sid, (lead + rin) * a.C + sp[k].c, ok ? sp[k].hi : 0, u);
+#pragma unroll
+                for (int j = 0; j < N; ++j) p.e[j] = (T)(u[j] >= d.least ? g[j] * d.scale : 0.f);
             }
-            if (a.dx) {
-                if (d.mode && ok && sp[k].any()) {
-                    uint32_t u[N];
-                    drop_words<N, COLS == ALIGNED>(d, sid, row * a.C + sp[k].c, sp[k].hi, u);
-#pragma unroll
-                    for (int j = 0; j < N; ++j) g[j] = u[j] >= d.least ? g[j] * d.scale : 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < N; ++j) p.e[j] = (T)g[j];
-                sp[k].store((T*)a.dx + row * a.C, ok, p);
-            }
+            sp[k].store((T*)a.dx + lead * a.C, ok && a.dx ? od[k] : NOWHERE, p);
             x[k] = xn[k];
             gy[k] = gn[k];
         }
+        ok = more;
     }
     if (!a.dw && !a.db) return;
 #pragma unroll
@@ -384,7 +404,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_bwd_k(NormArgs a, Drop
                     float t = which ? gb[k][j] : gw[k][j];
                     for (int o = G; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
                     if (lane < G && sp[k].mine(j))
-                        fold[((threadIdx.x >> 6) * NV + k) * 64 * N + (int)(sp[k].c - (long)k * G * N) + j] = t;
+                        fold[((threadIdx.x >> 6) * NV + k) * 64 * N + ((int)sp[k].c - k * G * N) + j] = t;
                 }
             __syncthreads();
             for (long c = threadIdx.x; c < a.C; c += 256) {
@@ -401,7 +421,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_bwd_k(NormArgs a, Drop
 #pragma unroll
                 for (int j = 0; j < N; ++j)
                     if (sp[k].mine(j)) {
-                        const long c = sp[k].c + j;
+                        const long c = (long)sp[k].c + j;
                         const float t = which ? gb[k][j] : gw[k][j];
                         if (gridDim.x > 1) out[c] = t;
                         else if (res) put_param<T>(res, a.wf32, c, t, a.accumulate);
@@ -434,6 +454,12 @@ __host__ __device__ static inline SplitPlan split_plan(long C, int size) {
     return s;
 }
 
+// first column that a tile's packs may touch (the last pack of a row may reach back into the tile before it)
+template <typename T>
+__device__ __forceinline__ long split_from(const SplitPlan& sp, long tile) {
+    return tile ? tile * sp.tile - Pack<T>::N : 0;
+}
+
 template <typename T, int COLS, bool RES, bool BWD>
 __global__ __launch_bounds__(256) void ln_split_stats_k(NormArgs a, Drop d, Chunk* __restrict__ st) {
     constexpr int N = Pack<T>::N;
@@ -444,6 +470,7 @@ __global__ __launch_bounds__(256) void ln_split_stats_k(NormArgs a, Drop d, Chun
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         double n = 0, mean = 0, m2 = 0, G = 0, H = 0;
         for (long t = blockIdx.x * sp.per; t < (blockIdx.x + 1) * sp.per && t < sp.tiles; ++t) {
+            const long from = split_from<T>(sp, t);
             Pack<T> x[SPLIT_NV];
             float g[SPLIT_NV][N];
             Span<T, COLS> c[SPLIT_NV];
@@ -451,14 +478,15 @@ __global__ __launch_bounds__(256) void ln_split_stats_k(NormArgs a, Drop d, Chun
 #pragma unroll
             for (int k = 0; k < SPLIT_NV; ++k) {
                 c[k] = Span<T, COLS>((t * SPLIT_NV + k) * 256 + threadIdx.x, a.C);
-                x[k] = c[k].load((const T*)a.x + row * a.ldx, true);
+                const uint32_t off = c[k].at(0, 0, (uint32_t)from);
+                x[k] = c[k].load((const T*)a.x + row * a.ldx + from, off);
                 if (RES) {
-                    const Pack<T> q = c[k].load((const T*)a.res + row * a.C, true);
-                    if (c[k].any()) x[k] = add_drop<T, COLS>(x[k], q, d, sid, row * a.C + c[k].c, c[k].hi);
-                    c[k].store((T*)a.s + row * a.C, true, x[k]);
+                    const Pack<T> q = c[k].load((const T*)a.res + row * a.C + from, off);
+                    x[k] = add_drop<T, COLS>(x[k], q, d, sid, row * a.C + c[k].c, c[k].hi);
+                    c[k].store((T*)a.s + row * a.C + from, off, x[k]);
                 }
                 if (BWD) {
-                    const Pack<T> q = c[k].load((const T*)a.dy + row * a.lddy, true);
+                    const Pack<T> q = c[k].load((const T*)a.dy + row * a.lddy + from, off);
                     c[k].params(a.weight, a.wf32, 1.f, g[k]);
 #pragma unroll
                     for (int j = 0; j < N; ++j) g[k][j] = c[k].mine(j) ? g[k][j] * (float)q.e[j] : 0.f;
@@ -555,15 +583,19 @@ template <typename T, int COLS>
 __global__ __launch_bounds__(256) void ln_split_fwd_k(NormArgs a, const Chunk* __restrict__ st) {
     constexpr int N = Pack<T>::N;
     const SplitPlan sp = split_plan(a.C, sizeof(T));
+    const long from = split_from<T>(sp, blockIdx.x);
+    Span<T, COLS> c[SPLIT_NV];
+    uint32_t off[SPLIT_NV];
+#pragma unroll
+    for (int k = 0; k < SPLIT_NV; ++k) {
+        c[k] = Span<T, COLS>((blockIdx.x * (long)SPLIT_NV + k) * 256 + threadIdx.x, a.C);
+        off[k] = c[k].at(0, 0, (uint32_t)from);
+    }
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        const T* src = a.s ? (const T*)a.s + row * a.C : (const T*)a.x + row * a.ldx;
-        Span<T, COLS> c[SPLIT_NV];
+        const T* src = (a.s ? (const T*)a.s + row * a.C : (const T*)a.x + row * a.ldx) + from;
         Pack<T> x[SPLIT_NV];
 #pragma unroll
-        for (int k = 0; k < SPLIT_NV; ++k) {
-            c[k] = Span<T, COLS>((blockIdx.x * (long)SPLIT_NV + k) * 256 + threadIdx.x, a.C);
-            x[k] = c[k].load(src, true);
-        }
+        for (int k = 0; k < SPLIT_NV; ++k) x[k] = c[k].load(src, off[k]);
         const RowStats s = join_chunks<false>(st + row * sp.chunks, sp, a.C, a.eps);
 #pragma unroll
         for (int k = 0; k < SPLIT_NV; ++k) {
@@ -573,7 +605,7 @@ __global__ __launch_bounds__(256) void ln_split_fwd_k(NormArgs a, const Chunk* _
             Pack<T> o;
 #pragma unroll
             for (int j = 0; j < N; ++j) o.e[j] = (T)((((float)x[k].e[j] - s.hi) - s.lo) * s.r * w[j] + b[j]);
-            c[k].store((T*)a.y + row * a.C, true, o);
+            c[k].store((T*)a.y + row * a.C + from, off[k], o);
         }
     }
 }
@@ -590,12 +622,15 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
     float w[SPLIT_NV][N], gw[SPLIT_NV][N], gb[SPLIT_NV][N];
     Span<T, COLS> c[SPLIT_NV];
     Pack<T> x[SPLIT_NV], gy[SPLIT_NV];
+    const long from = split_from<T>(sp, blockIdx.x);
+    uint32_t off[SPLIT_NV];
     long row = blockIdx.y;
 #pragma unroll
     for (int k = 0; k < SPLIT_NV; ++k) {
         c[k] = Span<T, COLS>((blockIdx.x * (long)SPLIT_NV + k) * 256 + threadIdx.x, a.C);
-        x[k] = c[k].load((const T*)a.x + row * a.ldx, row < a.rows);
-        gy[k] = c[k].load((const T*)a.dy + row * a.lddy, row < a.rows);
+        off[k] = c[k].at(0, 0, (uint32_t)from);
+        x[k] = c[k].load((const T*)a.x + row * a.ldx + from, off[k]);
+        gy[k] = c[k].load((const T*)a.dy + row * a.lddy + from, off[k]);
         c[k].params(a.weight, a.wf32, 1.f, w[k]);
 #pragma unroll
         for (int j = 0; j < N; ++j) gw[k][j] = gb[k][j] = 0.f;
@@ -613,12 +648,13 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
         }
         const RowStats s = stats[at];
         const long next = row + gridDim.y;
+        const bool more = next < a.rows;
         Pack<T> xn[SPLIT_NV], gn[SPLIT_NV], ds[SPLIT_NV];
 #pragma unroll
         for (int k = 0; k < SPLIT_NV; ++k) {
-            if (a.ds) ds[k] = c[k].load((const T*)a.ds + row * a.C, true);
-            xn[k] = c[k].load((const T*)a.x + next * a.ldx, next < a.rows);
-            gn[k] = c[k].load((const T*)a.dy + next * a.lddy, next < a.rows);
+            ds[k] = c[k].load((const T*)a.ds + row * a.C + from, a.ds ? off[k] : NOWHERE);
+            xn[k] = c[k].load((const T*)a.x + next * a.ldx + from, more ? off[k] : NOWHERE);
+            gn[k] = c[k].load((const T*)a.dy + next * a.lddy + from, more ? off[k] : NOWHERE);
         }
 #pragma unroll
         for (int k = 0; k < SPLIT_NV; ++k) {
@@ -629,28 +665,19 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
                 const float h = (((float)x[k].e[j] - s.hi) - s.lo) * s.r;
                 gw[k][j] += dy * h;
                 gb[k][j] += dy;
-                g[j] = s.r * (dy * w[k][j] - s.c1 - h * s.c2);
+                g[j] = s.r * (dy * w[k][j] - s.c1 - h * s.c2) + (float)ds[k].e[j];
             }
-            if (a.ds)
-#pragma unroll
-                for (int j = 0; j < N; ++j) g[j] += (float)ds[k].e[j];
             Pack<T> o;
-            if (a.dres) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) o.e[j] = (T)g[j];
-                c[k].store((T*)a.dres + row * a.C, true, o);
+            for (int j = 0; j < N; ++j) o.e[j] = (T)g[j];
+            c[k].store((T*)a.dres + row * a.C + from, a.dres ? off[k] : NOWHERE, o);
+            if (d.mode) {
+                uint32_t u[N];
+                drop_words<N, COLS == ALIGNED>(d, sid, row * a.C + c[k].c, c[k].hi, u);
+#pragma unroll
+                for (int j = 0; j < N; ++j) o.e[j] = (T)(u[j] >= d.least ? g[j] * d.scale : 0.f);
             }
-            if (a.dx) {
-                if (d.mode && c[k].any()) {
-                    uint32_t u[N];
-                    drop_words<N, COLS == ALIGNED>(d, sid, row * a.C + c[k].c, c[k].hi, u);
-#pragma unroll
-                    for (int j = 0; j < N; ++j) g[j] = u[j] >= d.least ? g[j] * d.scale : 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < N; ++j) o.e[j] = (T)g[j];
-                c[k].store((T*)a.dx + row * a.C, true, o);
-            }
+            c[k].store((T*)a.dx + row * a.C + from, a.dx ? off[k] : NOWHERE, o);
             x[k] = xn[k];
             gy[k] = gn[k];
         }
@@ -661,7 +688,7 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             if (!c[k].mine(j)) continue;
-            const long i = c[k].c + j;
+            const long i = (long)c[k].c + j;
             if (gridDim.y > 1) {
                 a.part[((long)blockIdx.y * 2 + 0) * a.C + i] = gw[k][j];
                 a.part[((long)blockIdx.y * 2 + 1) * a.C + i] = gb[k][j];
@@ -697,13 +724,15 @@ __global__ __launch_bounds__(1024) void ln_param_sum_k(const float* __restrict__
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
-// Which kernel: a function of the row length, the type and the direction alone, so that a row's result does not depend
-// on what is computed beside it.
+// Which kernel: a function of the row length and stride, the type and the direction alone, so that a row's result does
+// not depend on what is computed beside it.
 struct Form {
     int nt, nv, lg;         // nt 0: split
 };
-static Form ln_form(long C, int type, bool bwd) {
+static Form ln_form(long C, long ld, int type, bool bwd) {
     const long packs = cdiv(C, 16 / type_size(type));
+    // the wave form reaches all rows of a step (256 at most) with 31-bit offsets
+    if (packs <= 128 && ld >= (1L << 31) / (256 * 4)) return {256, 1, 6};
     if (packs <= 64) {
         int lg = 0;
         while ((1L << lg) < packs) ++lg;
@@ -735,8 +764,8 @@ static long ln_split_parts(long rows, const SplitPlan& sp) {
     if (p > rows / 8) p = rows / 8;
     return p < 1 ? 1 : p;
 }
-static size_t ln_ws_bytes(long rows, long C, int type, int bwd) {
-    const Form f = ln_form(C, type, bwd);
+static size_t ln_ws_bytes(long rows, long C, long ld, int type, int bwd) {
+    const Form f = ln_form(C, ld, type, bwd);
     if (f.nt == 0) {
         const SplitPlan sp = split_plan(C, type_size(type));
         const long parts = bwd ? ln_split_parts(rows, sp) : 1;
@@ -777,9 +806,9 @@ static int with_cols(Cols c, F f) {
 template <typename T, int COLS, bool RES>
 static void ln_fwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
     if (f.nt == 64 && f.nv == 1) ln_fwd_k<T, 1, 64, COLS, RES><<<g, 256, 0, st>>>(a, d);
+    else if (f.nt == 256) ln_fwd_k<T, 1, 256, COLS, RES><<<g, 256, 0, st>>>(a, d);
     else if constexpr (COLS != SHORT) {              // a row of less than a pack is one lane's
         if (f.nt == 64) ln_fwd_k<T, 2, 64, COLS, RES><<<g, 256, 0, st>>>(a, d);
-        else if (f.nt == 256) ln_fwd_k<T, 1, 256, COLS, RES><<<g, 256, 0, st>>>(a, d);
         else if (f.nt == 512) ln_fwd_k<T, 1, 512, COLS, RES><<<g, 512, 0, st>>>(a, d);
         else if (f.nv == 1) ln_fwd_k<T, 1, 1024, COLS, RES><<<g, 1024, 0, st>>>(a, d);
         else ln_fwd_k<T, 2, 1024, COLS, RES><<<g, 1024, 0, st>>>(a, d);
@@ -788,9 +817,9 @@ static void ln_fwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsig
 template <typename T, int COLS>
 static void ln_bwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
     if (f.nt == 64 && f.nv == 1) ln_bwd_k<T, 1, 64, COLS><<<g, 256, 0, st>>>(a, d);
+    else if (f.nt == 256) ln_bwd_k<T, 1, 256, COLS><<<g, 256, 0, st>>>(a, d);
     else if constexpr (COLS != SHORT) {
         if (f.nt == 128) ln_bwd_k<T, 1, 128, COLS><<<g, 128, 0, st>>>(a, d);
-        else if (f.nt == 256) ln_bwd_k<T, 1, 256, COLS><<<g, 256, 0, st>>>(a, d);
         else if (f.nt == 512) ln_bwd_k<T, 1, 512, COLS><<<g, 512, 0, st>>>(a, d);
         else if (f.nv == 1) ln_bwd_k<T, 1, 1024, COLS><<<g, 1024, 0, st>>>(a, d);
         else if constexpr (sizeof(T) == 4) ln_bwd_k<T, 2, 1024, COLS><<<g, 1024, 0, st>>>(a, d);
@@ -799,8 +828,8 @@ static void ln_bwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsig
 static unsigned grid_y(long n) { return (unsigned)(n < 65535 ? n : 65535); }
 
 static int ln_fwd(const char* what, NormArgs a, const Drop& d, bool res, int type, void* ws, size_t ws_bytes, hipStream_t st) {
-    if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, type, 0), ws, ws_bytes)) return rc;
-    const Form f = ln_form(a.C, type, false);
+    if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, a.ldx, type, 0), ws, ws_bytes)) return rc;
+    const Form f = ln_form(a.C, a.ldx, type, false);
     a.lg = f.lg;
     return with_type(type, [&](auto* t) {
         typedef typename std::remove_reference<decltype(*t)>::type T;
@@ -825,8 +854,8 @@ static int ln_fwd(const char* what, NormArgs a, const Drop& d, bool res, int typ
     });
 }
 static int ln_bwd(const char* what, NormArgs a, const Drop& d, int type, void* ws, size_t ws_bytes, hipStream_t st) {
-    if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, type, 1), ws, ws_bytes)) return rc;
-    const Form f = ln_form(a.C, type, true);
+    if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, std::max(a.ldx, a.lddy), type, 1), ws, ws_bytes)) return rc;
+    const Form f = ln_form(a.C, std::max(a.ldx, a.lddy), type, true);
     a.lg = f.lg;
     return with_type(type, [&](auto* t) {
         typedef typename std::remove_reference<decltype(*t)>::type T;
@@ -865,7 +894,8 @@ using namespace siv;
 
 extern "C" int siv_layer_norm_workspace(long rows, long C, int type, int backward, size_t* bytes) {
     SIV_CHECK_ARG(bytes && rows > 0 && C > 0 && known_type(type), "layer_norm_workspace: bad argument");
-    *bytes = ln_ws_bytes(rows, C, type, backward);
+    // (rows far apart take another kernel: enough for both)
+    *bytes = std::max(ln_ws_bytes(rows, C, C, type, backward), ln_ws_bytes(rows, C, 1L << 40, type, backward));
     return SIV_OK;
 }
 extern "C" int siv_layer_norm_fwd(const void* x, long ldx, const void* weight, const void* bias, int wtype, float eps,
