@@ -135,10 +135,19 @@ __device__ __forceinline__ void drawn_words(const Drop& d, uint64_t sid, uint64_
         v[4 * k + 3] = r.w;
     }
     if (!QUAD) {
+        // (values, not elements, are chosen between: a choice of elements becomes an array in LDS, and with it a read of
+        // the launch packet by every wave)
+        const bool one = i & 1, two = i & 2;
 #pragma unroll
-        for (int j = 0; j + 1 < CALLS * 4; ++j) v[j] = (i & 1) ? v[j + 1] : v[j];
+        for (int j = 0; j + 1 < CALLS * 4; ++j) {
+            const uint32_t here = v[j], next = v[j + 1];
+            v[j] = one ? next : here;
+        }
 #pragma unroll
-        for (int j = 0; j + 2 < CALLS * 4; ++j) v[j] = (i & 2) ? v[j + 2] : v[j];
+        for (int j = 0; j + 2 < CALLS * 4; ++j) {
+            const uint32_t here = v[j], next = v[j + 2];
+            v[j] = two ? next : here;
+        }
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) w[j] = v[j];

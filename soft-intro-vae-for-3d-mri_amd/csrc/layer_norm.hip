@@ -137,7 +137,7 @@ struct Span {
 #pragma unroll
             for (int j = 0; j < N; ++j) v.e[j] = off != NOWHERE && j < hi ? p[j] : (T)0.f;
         } else {
-            const words w = __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(base), off, 0, LAST && COLS == ALIGNED ? 2 : 0);
+            const words w = __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(base), off, 0, LAST ? 2 : 0);
             __builtin_memcpy(v.e, &w, 16);
         }
         return v;
@@ -151,8 +151,8 @@ struct Span {
         } else {
             words w;
             __builtin_memcpy(&w, v.e, 16);
-            // whole lines go out non-temporally: the L2, which a kernel's end writes back anyway, is left to the operands
-            __builtin_amdgcn_raw_buffer_store_b128(w, rows_rsrc(base), off, 0, COLS == ALIGNED ? 2 : 0);
+            // non-temporal: the L2, which a kernel's end writes back anyway, is left to the operands
+            __builtin_amdgcn_raw_buffer_store_b128(w, rows_rsrc(base), off, 0, 2);
         }
     }
     // this pack's columns of a parameter vector, in as few loads as the type allows
