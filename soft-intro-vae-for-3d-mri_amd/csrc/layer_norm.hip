@@ -54,11 +54,11 @@ __device__ __forceinline__ void lanes_sum(float (&v)[N], int lg) {
              v[k] = __uint_as_float(t[0]) + __uint_as_float(t[1]))
 #undef SIV_STEP
 }
-// Sums over the lanes that share a row: part of a wave (NT = 64), or a block of NT.  Two LDS buffers in turn: the
-// barrier of one sum also separates the readers of the sum before it from the writers of the next.
-template <int NT>
+// Sums over the lanes that share a row: part of a wave (NT = 64), or NT threads of a block of NT x R.  Two LDS buffers
+// in turn: the barrier of one sum also separates the readers of the sum before it from the writers of the next.
+template <int NT, int R>
 struct RowSum {
-    float4 (*sh)[NT / 64];
+    float4 (*sh)[R * NT / 64];
     int lg, turn;
     template <int N>
     __device__ __forceinline__ void operator()(float (&v)[N]) {
@@ -67,9 +67,9 @@ struct RowSum {
             return;
         }
         lanes_sum(v, 6);
-        float4* buf = sh[turn];
+        float4* buf = sh[turn] + (R > 1 ? threadIdx.x / NT * (NT / 64) : 0);
         if ((threadIdx.x & 63) == 0)
-            buf[threadIdx.x >> 6] = make_float4(v[0], N > 1 ? v[N > 1 ? 1 : 0] : 0.f, N > 2 ? v[N > 2 ? 2 : 0] : 0.f,
+            sh[turn][threadIdx.x >> 6] = make_float4(v[0], N > 1 ? v[N > 1 ? 1 : 0] : 0.f, N > 2 ? v[N > 2 ? 2 : 0] : 0.f,
                                                 N > 3 ? v[N > 3 ? 3 : 0] : 0.f);
         __syncthreads();
         float4 s = buf[0];
@@ -208,24 +208,24 @@ __device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res
 }
 
 // ---- rows held in registers -----------------------------------------------------------------------------------------
-// A row is spread over 2^lg lanes of a wave, 64 >> lg rows to a wave and four waves to a block (NT = 64), or over the
-// NT threads of a block; a lane holds NV packs of 16 bytes.  One pass over the data.  Blocks walk the rows in strides of
+// A row is spread over 2^lg lanes of a wave, 64 >> lg rows to a wave and four waves to a block (NT = 64), or over NT
+// threads, R rows to a block; a lane holds NV packs of 16 bytes.  One pass over the data.  Blocks walk the rows in strides of
 // the grid, so that weights and the parameters' gradients stay in registers; the next row is requested before the
 // present one is worked on.
-template <typename T, int NV, int NT, int COLS, bool RES>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_fwd_k(NormArgs a, Drop d) {
+template <typename T, int NV, int NT, int R, int COLS, bool RES>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
     constexpr bool AHEAD = NV > 1 || NT > 64;
-    __shared__ float4 sh[2][NT / 64];
-    RowSum<NT> row_sum{sh, a.lg, 0};
+    __shared__ float4 sh[2][R * NT / 64];
+    RowSum<NT, R> row_sum{sh, a.lg, 0};
     const int lane = threadIdx.x & 63;
     const int G = NT == 64 ? 1 << a.lg : NT;
-    const int sub = NT == 64 ? lane & (G - 1) : threadIdx.x;
-    const long per = NT == 64 ? 256 >> a.lg : 1;                      // rows of one block step
+    const int sub = NT == 64 ? lane & (G - 1) : threadIdx.x % NT;
+    const long per = NT == 64 ? 256 >> a.lg : R;                      // rows of one block step
     const long step = (long)gridDim.x * per;
     const uint64_t sid = RES ? drop_sid(d) : 0;
     const float invC = 1.0f / (float)a.C;
-    const int rin = NT == 64 ? threadIdx.x >> a.lg : 0;               // this lane's row within the step
+    const int rin = NT == 64 ? threadIdx.x >> a.lg : threadIdx.x / NT;   // this lane's row within the step
     Span<T, COLS> sp[NV];
     float w[NV][N], b[NV][N];
     uint32_t ox[NV], od[NV];                                          // offsets in x, and in the dense tensors
@@ -295,21 +295,22 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_fwd_k(NormArgs a, Drop
 
 // The same rows backward.  Each lane sums dy h and dy of its columns over the rows it sees; a block's sums go to
 // a.part, or straight to the results where there is one block.
-template <typename T, int NV, int NT, int COLS>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_bwd_k(NormArgs a, Drop d) {
+template <typename T, int NV, int NT, int R, int COLS>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_bwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
     constexpr bool LAST = NT == 64;
-    __shared__ float4 sh[2][NT / 64];
-    __shared__ float fold[NT == 64 ? 4 * 64 * NV * N : 1];
-    RowSum<NT> row_sum{sh, a.lg, 0};
+    __shared__ float4 sh[2][R * NT / 64];
+    constexpr int ROWS = NT == 64 ? 4 : R, WIDE = NT * NV * N;    // sums to join at the end, columns of one
+    __shared__ float fold[ROWS * WIDE];
+    RowSum<NT, R> row_sum{sh, a.lg, 0};
     const int lane = threadIdx.x & 63;
     const int G = NT == 64 ? 1 << a.lg : NT;
-    const int sub = NT == 64 ? lane & (G - 1) : threadIdx.x;
-    const long per = NT == 64 ? 256 >> a.lg : 1;
+    const int sub = NT == 64 ? lane & (G - 1) : threadIdx.x % NT;
+    const long per = NT == 64 ? 256 >> a.lg : R;
     const long step = (long)gridDim.x * per;
     const uint64_t sid = drop_sid(d);
     const float invC = 1.0f / (float)a.C;
-    const int rin = NT == 64 ? threadIdx.x >> a.lg : 0;
+    const int rin = NT == 64 ? threadIdx.x >> a.lg : threadIdx.x / NT;
     Span<T, COLS> sp[NV];
     float w[NV][N], gw[NV][N], gb[NV][N];
     uint32_t ox[NV], oy[NV], od[NV];
@@ -395,38 +396,26 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void ln_bwd_k(NormArgs a, Drop
     for (int which = 0; which < 2; ++which) {
         float* out = a.part + ((long)blockIdx.x * 2 + which) * a.C;
         void* res = which ? a.db : a.dw;
-        if (NT == 64) {
-            // rows of one wave that share columns, then the four waves
+        const int mine = NT == 64 ? threadIdx.x >> 6 : rin;
+        // wave form: rows of one wave that share columns; then the waves or rows of the block
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    float t = which ? gb[k][j] : gw[k][j];
+            for (int j = 0; j < N; ++j) {
+                float t = which ? gb[k][j] : gw[k][j];
+                if (NT == 64)
                     for (int o = G; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
-                    if (lane < G && sp[k].mine(j))
-                        fold[((threadIdx.x >> 6) * NV + k) * 64 * N + ((int)sp[k].c - k * G * N) + j] = t;
-                }
-            __syncthreads();
-            for (long c = threadIdx.x; c < a.C; c += 256) {
-                const int k = (int)(c / (G * N)), o = (int)(c - (long)k * G * N);
-                const float t = (fold[(0 * NV + k) * 64 * N + o] + fold[(1 * NV + k) * 64 * N + o]) +
-                                (fold[(2 * NV + k) * 64 * N + o] + fold[(3 * NV + k) * 64 * N + o]);
-                if (gridDim.x > 1) out[c] = t;
-                else if (res) put_param<T>(res, a.wf32, c, t, a.accumulate);
+                if ((NT > 64 || lane < G) && sp[k].mine(j)) fold[mine * WIDE + (int)sp[k].c + j] = t;
             }
-            __syncthreads();
-        } else {
+        __syncthreads();
+        for (int c = threadIdx.x; c < (int)a.C; c += blockDim.x) {
+            float t = fold[c];
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (sp[k].mine(j)) {
-                        const long c = (long)sp[k].c + j;
-                        const float t = which ? gb[k][j] : gw[k][j];
-                        if (gridDim.x > 1) out[c] = t;
-                        else if (res) put_param<T>(res, a.wf32, c, t, a.accumulate);
-                    }
+            for (int i = 1; i < ROWS; ++i) t += fold[i * WIDE + c];
+            if (gridDim.x > 1) out[c] = t;
+            else if (res) put_param<T>(res, a.wf32, c, t, a.accumulate);
         }
+        __syncthreads();
     }
 }
 
@@ -464,7 +453,7 @@ template <typename T, int COLS, bool RES, bool BWD>
 __global__ __launch_bounds__(256) void ln_split_stats_k(NormArgs a, Drop d, Chunk* __restrict__ st) {
     constexpr int N = Pack<T>::N;
     __shared__ float4 sh[2][4];
-    RowSum<256> row_sum{sh, 6, 0};
+    RowSum<256, 1> row_sum{sh, 6, 0};
     const SplitPlan sp = split_plan(a.C, sizeof(T));
     const uint64_t sid = RES ? drop_sid(d) : 0;
     for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -728,6 +717,8 @@ __global__ __launch_bounds__(1024) void ln_param_sum_k(const float* __restrict__
 // not depend on what is computed beside it.
 struct Form {
     int nt, nv, lg;         // nt 0: split
+    int rows() const { return nt == 64 ? 256 >> lg : nt == 128 ? 4 : nt == 256 ? 2 : 1; }      // of one block step
+    int threads() const { return nt == 64 ? 256 : nt * rows(); }
 };
 static Form ln_form(long C, long ld, int type, bool bwd) {
     const long packs = cdiv(C, 16 / type_size(type));
@@ -746,15 +737,13 @@ static Form ln_form(long C, long ld, int type, bool bwd) {
     return {0, 0, 0};
 }
 static long ln_blocks(long rows, const Form& f, bool bwd) {
-    const long per = f.nt == 64 ? 256 >> f.lg : 1;
-    const long steps = cdiv(rows, per);
-    const int threads = f.nt == 64 ? 256 : f.nt;
+    const long steps = cdiv(rows, f.rows());
     if (!bwd) {
-        const long cap = f.nt > 64 ? 2048 * 256L / threads : f.nv == 2 ? 8192 : 1L << 20;
+        const long cap = f.nt > 64 ? 2048 * 256L / f.threads() : f.nv == 2 ? 8192 : 1L << 20;
         return steps < cap ? steps : cap;
     }
     if (steps <= 4) return 1;                        // the parameters' gradients in one launch
-    const long cap = f.nt == 64 ? 768 : 1024 * 256L / threads;
+    const long cap = (f.nt == 64 ? 768 : 1024) * 256L / f.threads();
     const long b = steps / 4 > 256 ? steps / 4 : 256;
     return std::min(std::min(b, cap), steps);
 }
@@ -805,24 +794,24 @@ static int with_cols(Cols c, F f) {
 }
 template <typename T, int COLS, bool RES>
 static void ln_fwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
-    if (f.nt == 64 && f.nv == 1) ln_fwd_k<T, 1, 64, COLS, RES><<<g, 256, 0, st>>>(a, d);
-    else if (f.nt == 256) ln_fwd_k<T, 1, 256, COLS, RES><<<g, 256, 0, st>>>(a, d);
+    if (f.nt == 64 && f.nv == 1) ln_fwd_k<T, 1, 64, 1, COLS, RES><<<g, 256, 0, st>>>(a, d);
+    else if (f.nt == 256) ln_fwd_k<T, 1, 256, 2, COLS, RES><<<g, 512, 0, st>>>(a, d);
     else if constexpr (COLS != SHORT) {              // a row of less than a pack is one lane's
-        if (f.nt == 64) ln_fwd_k<T, 2, 64, COLS, RES><<<g, 256, 0, st>>>(a, d);
-        else if (f.nt == 512) ln_fwd_k<T, 1, 512, COLS, RES><<<g, 512, 0, st>>>(a, d);
-        else if (f.nv == 1) ln_fwd_k<T, 1, 1024, COLS, RES><<<g, 1024, 0, st>>>(a, d);
-        else ln_fwd_k<T, 2, 1024, COLS, RES><<<g, 1024, 0, st>>>(a, d);
+        if (f.nt == 64) ln_fwd_k<T, 2, 64, 1, COLS, RES><<<g, 256, 0, st>>>(a, d);
+        else if (f.nt == 512) ln_fwd_k<T, 1, 512, 1, COLS, RES><<<g, 512, 0, st>>>(a, d);
+        else if (f.nv == 1) ln_fwd_k<T, 1, 1024, 1, COLS, RES><<<g, 1024, 0, st>>>(a, d);
+        else ln_fwd_k<T, 2, 1024, 1, COLS, RES><<<g, 1024, 0, st>>>(a, d);
     }
 }
 template <typename T, int COLS>
 static void ln_bwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
-    if (f.nt == 64 && f.nv == 1) ln_bwd_k<T, 1, 64, COLS><<<g, 256, 0, st>>>(a, d);
-    else if (f.nt == 256) ln_bwd_k<T, 1, 256, COLS><<<g, 256, 0, st>>>(a, d);
+    if (f.nt == 64 && f.nv == 1) ln_bwd_k<T, 1, 64, 1, COLS><<<g, 256, 0, st>>>(a, d);
+    else if (f.nt == 256) ln_bwd_k<T, 1, 256, 2, COLS><<<g, 512, 0, st>>>(a, d);
     else if constexpr (COLS != SHORT) {
-        if (f.nt == 128) ln_bwd_k<T, 1, 128, COLS><<<g, 128, 0, st>>>(a, d);
-        else if (f.nt == 512) ln_bwd_k<T, 1, 512, COLS><<<g, 512, 0, st>>>(a, d);
-        else if (f.nv == 1) ln_bwd_k<T, 1, 1024, COLS><<<g, 1024, 0, st>>>(a, d);
-        else if constexpr (sizeof(T) == 4) ln_bwd_k<T, 2, 1024, COLS><<<g, 1024, 0, st>>>(a, d);
+        if (f.nt == 128) ln_bwd_k<T, 1, 128, 4, COLS><<<g, 512, 0, st>>>(a, d);
+        else if (f.nt == 512) ln_bwd_k<T, 1, 512, 1, COLS><<<g, 512, 0, st>>>(a, d);
+        else if (f.nv == 1) ln_bwd_k<T, 1, 1024, 1, COLS><<<g, 1024, 0, st>>>(a, d);
+        else if constexpr (sizeof(T) == 4) ln_bwd_k<T, 2, 1024, 1, COLS><<<g, 1024, 0, st>>>(a, d);
     }
 }
 static unsigned grid_y(long n) { return (unsigned)(n < 65535 ? n : 65535); }
