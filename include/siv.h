@@ -424,7 +424,7 @@ int siv_act_dropout_bwd(const float* dout, const float* x, const uint8_t* keep, 
  *    all arithmetic are fp32, results are rounded to nearest even once.  weight / bias (and their gradients) are
  *    [C] of `wtype`: SIV_F32 or `type`; either may be NULL (factor 1 / offset 0).
  *  - x and dy are rows of C consecutive elements, ldx / lddy elements apart (>= C); y and dx are dense.  Any
- *    alignment of the element type is accepted.  x must not overlap y / dx.
+ *    alignment of the element type is accepted.  No result may overlap an input or another result.
  *  - forward keeps nothing for backward: the statistics are formed again from x.
  *  - dx, dweight, dbias may be NULL; accumulate != 0 adds into dweight / dbias.  Their sums have a fixed order.
  *  - ws: siv_layer_norm_workspace writes the bytes the forward (backward = 0) or backward (1) call of that size
@@ -437,7 +437,7 @@ int siv_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, const
                        long C, void* ws, size_t ws_bytes, siv_stream_t stream);
 /* The closing step of a residual branch in one pass: s = residual + dropout(x), held in `type`, and
  * y = layer_norm(s) of what is held.  All tensors are dense [rows][C].  Dropout as in siv_dropout_fwd (element i of
- * x is drawn at index i); p == 0 with keep == NULL adds x itself.
+ * x is drawn at index i); p == 0 with keep == NULL adds x itself.  No result may overlap an input or another result.
  * _bwd: dy and ds (NULL = zero) are the gradients of y and s; dresidual = ds + the norm's input gradient,
  * dx = dropout's backward of it; any of the four results may be NULL.  Workspace as for siv_layer_norm_*. */
 int siv_add_layer_norm_fwd(const void* x, const void* residual, const uint8_t* keep, uint64_t seed,

@@ -286,10 +286,19 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, 
 #pragma unroll
             for (int j = 0; j < N; ++j) p.e[j] = (T)((v[k][j] - delta) * r * w[k][j] + b[k][j]);
             sp[k].store((T*)a.y + lead * a.C, ok ? od[k] : NOWHERE, p);
-            x[k] = AHEAD ? xn[k] : sp[k].load((const T*)a.x + (lead + step) * a.ldx, more ? ox[k] : NOWHERE);
-            if (RES) q[k] = AHEAD ? qn[k] : sp[k].load((const T*)a.res + (lead + step) * a.C, more ? od[k] : NOWHERE);
+            if (AHEAD) {
+                x[k] = xn[k];
+                if (RES) q[k] = qn[k];
+            }
         }
         ok = more;
+        if (AHEAD) continue;
+        if (lead + step >= a.rows) break;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            x[k] = sp[k].load((const T*)a.x + (lead + step) * a.ldx, more ? ox[k] : NOWHERE);
+            if (RES) q[k] = sp[k].load((const T*)a.res + (lead + step) * a.C, more ? od[k] : NOWHERE);
+        }
     }
 }
 
@@ -722,19 +731,24 @@ struct Form {
 };
 static Form ln_form(long C, long ld, int type, bool bwd) {
     const long packs = cdiv(C, 16 / type_size(type));
-    // the wave form reaches all rows of a step (256 at most) with 31-bit offsets
-    if (packs <= 128 && ld >= (1L << 31) / (256 * 4)) return {256, 1, 6};
+    Form f = {0, 0, 0};
     if (packs <= 64) {
-        int lg = 0;
-        while ((1L << lg) < packs) ++lg;
-        return {64, 1, lg};
+        f = {64, 1, 0};
+        while ((1L << f.lg) < packs) ++f.lg;
+    } else if (packs <= 128) {
+        f = bwd ? Form{128, 1, 6} : Form{64, 2, 6};
+    } else if (packs <= 256) {
+        f = {256, 1, 6};
+    } else if (packs <= 512) {
+        f = {512, 1, 6};
+    } else if (packs <= 1024) {
+        f = {1024, 1, 6};
+    } else if (packs <= 2048 && (!bwd || type == SIV_F32)) {
+        f = {1024, 2, 6};
     }
-    if (packs <= 128) return bwd ? Form{128, 1, 6} : Form{64, 2, 6};
-    if (packs <= 256) return {256, 1, 6};
-    if (packs <= 512) return {512, 1, 6};
-    if (packs <= 1024) return {1024, 1, 6};
-    if (packs <= 2048 && (!bwd || type == SIV_F32)) return {1024, 2, 6};
-    return {0, 0, 0};
+    // the rows of a step are reached with 31-bit offsets: rows very far apart go one to a step
+    if (f.nt && f.rows() > 1 && ld >= (1L << 31) / (f.rows() * 4L)) f = {512, 1, 6};
+    return f;
 }
 static long ln_blocks(long rows, const Form& f, bool bwd) {
     const long steps = cdiv(rows, f.rows());
@@ -795,10 +809,10 @@ static int with_cols(Cols c, F f) {
 template <typename T, int COLS, bool RES>
 static void ln_fwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
     if (f.nt == 64 && f.nv == 1) ln_fwd_k<T, 1, 64, 1, COLS, RES><<<g, 256, 0, st>>>(a, d);
-    else if (f.nt == 256) ln_fwd_k<T, 1, 256, 2, COLS, RES><<<g, 512, 0, st>>>(a, d);
-    else if constexpr (COLS != SHORT) {              // a row of less than a pack is one lane's
+    else if (f.nt == 512) ln_fwd_k<T, 1, 512, 1, COLS, RES><<<g, 512, 0, st>>>(a, d);
+    else if constexpr (COLS != SHORT) {              // (a row of less than a pack takes one of the two above)
         if (f.nt == 64) ln_fwd_k<T, 2, 64, 1, COLS, RES><<<g, 256, 0, st>>>(a, d);
-        else if (f.nt == 512) ln_fwd_k<T, 1, 512, 1, COLS, RES><<<g, 512, 0, st>>>(a, d);
+        else if (f.nt == 256) ln_fwd_k<T, 1, 256, 2, COLS, RES><<<g, 512, 0, st>>>(a, d);
         else if (f.nv == 1) ln_fwd_k<T, 1, 1024, 1, COLS, RES><<<g, 1024, 0, st>>>(a, d);
         else ln_fwd_k<T, 2, 1024, 1, COLS, RES><<<g, 1024, 0, st>>>(a, d);
     }
@@ -806,10 +820,10 @@ static void ln_fwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsig
 template <typename T, int COLS>
 static void ln_bwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
     if (f.nt == 64 && f.nv == 1) ln_bwd_k<T, 1, 64, 1, COLS><<<g, 256, 0, st>>>(a, d);
-    else if (f.nt == 256) ln_bwd_k<T, 1, 256, 2, COLS><<<g, 512, 0, st>>>(a, d);
+    else if (f.nt == 512) ln_bwd_k<T, 1, 512, 1, COLS><<<g, 512, 0, st>>>(a, d);
     else if constexpr (COLS != SHORT) {
         if (f.nt == 128) ln_bwd_k<T, 1, 128, 4, COLS><<<g, 512, 0, st>>>(a, d);
-        else if (f.nt == 512) ln_bwd_k<T, 1, 512, 1, COLS><<<g, 512, 0, st>>>(a, d);
+        else if (f.nt == 256) ln_bwd_k<T, 1, 256, 2, COLS><<<g, 512, 0, st>>>(a, d);
         else if (f.nv == 1) ln_bwd_k<T, 1, 1024, 1, COLS><<<g, 1024, 0, st>>>(a, d);
         else if constexpr (sizeof(T) == 4) ln_bwd_k<T, 2, 1024, 1, COLS><<<g, 1024, 0, st>>>(a, d);
     }

@@ -152,6 +152,20 @@ def test_row_views_take_no_copy(hip):
 
 
 @pytest.mark.parametrize("dtype", N.DTYPES, ids=N.IDS)
+@pytest.mark.parametrize("C", [1, 3, 8, 100, 700])
+def test_layer_norm_rows_far_apart(C, dtype):
+    """Rows 2^21 and more elements apart (a step of many rows no longer spans 31-bit offsets), and one pair 2^30 apart."""
+    w, b = (1 + 0.2 * rnd(3, C)).cuda(), rnd(4, C).cuda()
+    for R, ld in ((9, (1 << 21) + 8), (5, (1 << 21) - 3), (2, (1 << 30) + 1)):
+        base, dbase = (torch.zeros((R - 1) * ld + C + 64, dtype=dtype, device="cuda") for _ in range(2))
+        x, dy = (t[3:].as_strided((R, C), (ld, 1)) for t in (base, dbase))
+        x.copy_(rnd(1, R, C, scale=1.5, offset=0.5, dtype=dtype))
+        dy.copy_(rnd(2, R, C, dtype=dtype))
+        check_norm(x, dy, w, b, 1e-5, dtype, torch.float32)
+        del base, dbase, x, dy
+
+
+@pytest.mark.parametrize("dtype", N.DTYPES, ids=N.IDS)
 def test_layer_norm_stays_in_its_rows(dtype):
     """Results of short calls inside larger buffers: nothing before, behind or between is written."""
     from siv import backend as sb
@@ -292,6 +306,23 @@ def test_a_changed_input_is_noticed(hip):
     s.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+def test_leaf_gradients_are_separate(hip):
+    """x and residual share one gradient where nothing is dropped; their .grad tensors do not share memory."""
+    o = ops()
+    for f in (lambda x, r: o.add_layer_norm(x, r)[0], lambda x, r: o.add_layer_norm(x, r)[1],
+              lambda x, r: o.dropout(x, key(), 0.5, residual=r)):
+        x, r = rnd(1, 6, 40).cuda().requires_grad_(), rnd(2, 6, 40).cuda().requires_grad_()
+        up = rnd(3, 6, 40).cuda()
+        keep = up.clone()
+        f(x, r).backward(up)
+        want = r.grad.clone()
+        x.grad.zero_()
+        assert torch.equal(r.grad, want) and torch.equal(up, keep)
+        f(x, r).backward(up)
+        assert torch.equal(r.grad, 2 * want)
+        assert torch.equal(up, keep)
 
 
 def test_frozen_parameters_and_inputs(hip):
