@@ -120,6 +120,8 @@ struct Span {
         }
     }
     __device__ __forceinline__ bool any() const { return lo < hi; }
+    // whether some lane of the wave holds part of a pack: only there do sums look at single elements
+    __device__ __forceinline__ bool ragged() const { return COLS != ALIGNED && __any(any() && hi - lo < N); }
     __device__ __forceinline__ bool mine(int j) const {
         return COLS == ALIGNED ? hi > 0 : COLS == OVERLAP ? j >= lo : j < hi;
     }
@@ -190,6 +192,39 @@ __device__ __forceinline__ void put_param(void* out, int f32, long c, float v, i
     else ((T*)out)[c] = (T)(accumulate ? (float)((T*)out)[c] + v : v);
 }
 
+// What one pack adds to a row's sums: sum x; or, of d = x - m0 and g = dy w, sum d, sum d^2, sum g, sum g d.
+template <typename T, int COLS>
+__device__ __forceinline__ float pack_sum(const Span<T, COLS>& sp, bool ragged, const Pack<T>& x) {
+    float s = 0.f;
+    if (ragged) {
+#pragma unroll
+        for (int j = 0; j < Pack<T>::N; ++j) s += sp.mine(j) ? (float)x.e[j] : 0.f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < Pack<T>::N; ++j) s += (float)x.e[j];
+    }
+    return sp.any() ? s : 0.f;
+}
+template <typename T, int COLS, bool BWD>
+__device__ __forceinline__ void pack_sums(const Span<T, COLS>& sp, bool ragged, const float* d, const float* g,
+                                          float (&m)[4]) {
+    constexpr int N = Pack<T>::N;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float dj = !ragged || sp.mine(j) ? d[j] : 0.f;
+        s[0] += dj;
+        s[1] += dj * dj;
+        if (BWD) {
+            const float gj = !ragged || sp.mine(j) ? g[j] : 0.f;
+            s[2] += gj;
+            s[3] += gj * dj;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < (BWD ? 4 : 2); ++i) m[i] += sp.any() ? s[i] : 0.f;
+}
+
 // residual + dropout(x) of one pack from element i on, as it is held
 template <typename T, int COLS>
 __device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res, const Drop& d, uint64_t sid, long i, int hi) {
@@ -229,12 +264,14 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, 
     Span<T, COLS> sp[NV];
     float w[NV][N], b[NV][N];
     uint32_t ox[NV], od[NV];                                          // offsets in x, and in the dense tensors
+    bool ragged[NV];
     long lead = (long)blockIdx.x * per;                               // first row of the step
     bool ok = rin < a.rows - lead;
     Pack<T> x[NV], q[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         sp[k] = Span<T, COLS>(k * G + sub, a.C);
+        ragged[k] = sp[k].ragged();
         ox[k] = sp[k].at(rin, a.ldx);
         od[k] = sp[k].at(rin, a.C);
         x[k] = sp[k].load((const T*)a.x + lead * a.ldx, ok ? ox[k] : NOWHERE);
@@ -259,32 +296,26 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, 
                 x[k] = add_drop<T, COLS>(x[k], q[k], d, sid, (lead + rin) * a.C + sp[k].c, ok ? sp[k].hi : 0);
                 sp[k].store((T*)a.s + lead * a.C, ok ? od[k] : NOWHERE, x[k]);
             }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                v[k][j] = sp[k].mine(j) ? (float)x[k].e[j] : 0.f;
-                s1[0] += v[k][j];
-            }
+            s1[0] += pack_sum(sp[k], ragged[k], x[k]);
         }
         row_sum(s1);
         const float m0 = s1[0] * invC;
-        float m[2] = {0.f, 0.f};
+        float m4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                v[k][j] = (float)x[k].e[j] - m0;
-                const float t = sp[k].mine(j) ? v[k][j] : 0.f;
-                m[0] += t;
-                m[1] += t * t;
-            }
+            for (int j = 0; j < N; ++j) v[k][j] = (float)x[k].e[j] - m0;
+            pack_sums<T, COLS, false>(sp[k], ragged[k], v[k], nullptr, m4);
+        }
+        float m[2] = {m4[0], m4[1]};
         row_sum(m);
         const float delta = m[0] * invC;
-        const float r = rsqrtf(fmaxf(m[1] * invC - delta * delta, 0.f) + a.eps);
+        const float r = rsqrtf(fmaxf(m[1] * invC - delta * delta, 0.f) + a.eps), dr = -delta * r;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             Pack<T> p;
 #pragma unroll
-            for (int j = 0; j < N; ++j) p.e[j] = (T)((v[k][j] - delta) * r * w[k][j] + b[k][j]);
+            for (int j = 0; j < N; ++j) p.e[j] = (T)((v[k][j] * r + dr) * w[k][j] + b[k][j]);
             sp[k].store((T*)a.y + lead * a.C, ok ? od[k] : NOWHERE, p);
             if (AHEAD) {
                 x[k] = xn[k];
@@ -304,7 +335,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, 
 
 // The same rows backward.  Each lane sums dy h and dy of its columns over the rows it sees; a block's sums go to
 // a.part, or straight to the results where there is one block.
-template <typename T, int NV, int NT, int R, int COLS>
+template <typename T, int NV, int NT, int R, int COLS, bool RES>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_bwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
     constexpr bool LAST = NT == 64;
@@ -317,18 +348,20 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_bwd_k(NormArgs a, 
     const int sub = NT == 64 ? lane & (G - 1) : threadIdx.x % NT;
     const long per = NT == 64 ? 256 >> a.lg : R;
     const long step = (long)gridDim.x * per;
-    const uint64_t sid = drop_sid(d);
+    const uint64_t sid = RES ? drop_sid(d) : 0;
     const float invC = 1.0f / (float)a.C;
     const int rin = NT == 64 ? threadIdx.x >> a.lg : threadIdx.x / NT;
     Span<T, COLS> sp[NV];
     float w[NV][N], gw[NV][N], gb[NV][N];
     uint32_t ox[NV], oy[NV], od[NV];
+    bool ragged[NV];
     long lead = (long)blockIdx.x * per;
     bool ok = rin < a.rows - lead;
     Pack<T> x[NV], gy[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         sp[k] = Span<T, COLS>(k * G + sub, a.C);
+        ragged[k] = sp[k].ragged();
         ox[k] = sp[k].at(rin, a.ldx);
         oy[k] = sp[k].at(rin, a.lddy);
         od[k] = sp[k].at(rin, a.C);
@@ -343,56 +376,53 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_bwd_k(NormArgs a, 
         Pack<T> xn[NV], gn[NV], ds[NV];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            ds[k] = sp[k].template load<LAST>((const T*)a.ds + lead * a.C, ok && a.ds ? od[k] : NOWHERE);
+            if (RES) ds[k] = sp[k].template load<LAST>((const T*)a.ds + lead * a.C, ok && a.ds ? od[k] : NOWHERE);
             xn[k] = sp[k].template load<LAST>((const T*)a.x + (lead + step) * a.ldx, more ? ox[k] : NOWHERE);
             gn[k] = sp[k].template load<LAST>((const T*)a.dy + (lead + step) * a.lddy, more ? oy[k] : NOWHERE);
         }
         float s1[1] = {0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int j = 0; j < N; ++j) s1[0] += sp[k].mine(j) ? (float)x[k].e[j] : 0.f;
+        for (int k = 0; k < NV; ++k) s1[0] += pack_sum(sp[k], ragged[k], x[k]);
         row_sum(s1);
         const float m0 = s1[0] * invC;
         float m[4] = {0.f, 0.f, 0.f, 0.f};
-        float v[NV][N];
+        float v[NV][N], g[NV][N];
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 v[k][j] = (float)x[k].e[j] - m0;
-                const float t = sp[k].mine(j) ? v[k][j] : 0.f;
-                const float g = sp[k].mine(j) ? (float)gy[k].e[j] * w[k][j] : 0.f;
-                m[0] += t;
-                m[1] += t * t;
-                m[2] += g;
-                m[3] += g * t;
+                g[k][j] = (float)gy[k].e[j] * w[k][j];
             }
+            pack_sums<T, COLS, true>(sp[k], ragged[k], v[k], g[k], m);
+        }
         row_sum(m);
         const float delta = m[0] * invC;
         float r = rsqrtf(fmaxf(m[1] * invC - delta * delta, 0.f) + a.eps);
         if (!ok) r = 0.f;                    // lanes without a row add nothing, whatever eps is
-        const float c1 = m[2] * invC, c2 = (m[3] - delta * m[2]) * r * invC;
+        // h = v r + dr;  dx = g r - c1 r - h c2 r
+        const float dr = -delta * r, k1 = -m[2] * invC * r, k2 = -(m[3] - delta * m[2]) * r * invC * r;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            float g[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float dy = (float)gy[k].e[j];
-                const float h = (v[k][j] - delta) * r;
+                const float dy = (float)gy[k].e[j], h = v[k][j] * r + dr;
                 gw[k][j] += dy * h;
                 gb[k][j] += dy;
-                g[j] = r * (dy * w[k][j] - c1 - h * c2) + (float)ds[k].e[j];
+                g[k][j] = h * k2 + (g[k][j] * r + k1);
+                if (RES) g[k][j] += (float)ds[k].e[j];
             }
             Pack<T> p;
 #pragma unroll
-            for (int j = 0; j < N; ++j) p.e[j] = (T)g[j];
-            sp[k].store((T*)a.dres + lead * a.C, ok && a.dres ? od[k] : NOWHERE, p);
-            if (d.mode) {
-                uint32_t u[N];
-                drop_words<N, COLS == ALIGNED>(d, sid, (lead + rin) * a.C + sp[k].c, ok ? sp[k].hi : 0, u);
+            for (int j = 0; j < N; ++j) p.e[j] = (T)g[k][j];
+            if (RES) {
+                sp[k].store((T*)a.dres + lead * a.C, ok && a.dres ? od[k] : NOWHERE, p);
+                if (d.mode) {
+                    uint32_t u[N];
+                    drop_words<N, COLS == ALIGNED>(d, sid, (lead + rin) * a.C + sp[k].c, ok ? sp[k].hi : 0, u);
 #pragma unroll
-                for (int j = 0; j < N; ++j) p.e[j] = (T)(u[j] >= d.least ? g[j] * d.scale : 0.f);
+                    for (int j = 0; j < N; ++j) p.e[j] = (T)(u[j] >= d.least ? g[k][j] * d.scale : 0.f);
+                }
             }
             sp[k].store((T*)a.dx + lead * a.C, ok && a.dx ? od[k] : NOWHERE, p);
             x[k] = xn[k];
@@ -602,7 +632,7 @@ __global__ __launch_bounds__(256) void ln_split_fwd_k(NormArgs a, const Chunk* _
             c[k].params(a.bias, a.wf32, 0.f, b);
             Pack<T> o;
 #pragma unroll
-            for (int j = 0; j < N; ++j) o.e[j] = (T)((((float)x[k].e[j] - s.hi) - s.lo) * s.r * w[j] + b[j]);
+            for (int j = 0; j < N; ++j) o.e[j] = (T)((((float)x[k].e[j] - s.hi) * s.r - s.lo * s.r) * w[j] + b[j]);
             c[k].store((T*)a.y + row * a.C + from, off[k], o);
         }
     }
@@ -645,6 +675,7 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
             __syncthreads();
         }
         const RowStats s = stats[at];
+        const float dr = -s.lo * s.r, k1 = -s.c1 * s.r, k2 = -s.c2 * s.r;
         const long next = row + gridDim.y;
         const bool more = next < a.rows;
         Pack<T> xn[SPLIT_NV], gn[SPLIT_NV], ds[SPLIT_NV];
@@ -660,10 +691,10 @@ __global__ __launch_bounds__(256) void ln_split_bwd_k(NormArgs a, Drop d, const 
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float dy = (float)gy[k].e[j];
-                const float h = (((float)x[k].e[j] - s.hi) - s.lo) * s.r;
+                const float h = ((float)x[k].e[j] - s.hi) * s.r + dr;
                 gw[k][j] += dy * h;
                 gb[k][j] += dy;
-                g[j] = s.r * (dy * w[k][j] - s.c1 - h * s.c2) + (float)ds[k].e[j];
+                g[j] = h * k2 + (dy * w[k][j] * s.r + k1) + (float)ds[k].e[j];
             }
             Pack<T> o;
 #pragma unroll
@@ -817,15 +848,15 @@ static void ln_fwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsig
         else ln_fwd_k<T, 2, 1024, 1, COLS, RES><<<g, 1024, 0, st>>>(a, d);
     }
 }
-template <typename T, int COLS>
+template <typename T, int COLS, bool RES>
 static void ln_bwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsigned g, hipStream_t st) {
-    if (f.nt == 64 && f.nv == 1) ln_bwd_k<T, 1, 64, 1, COLS><<<g, 256, 0, st>>>(a, d);
-    else if (f.nt == 512) ln_bwd_k<T, 1, 512, 1, COLS><<<g, 512, 0, st>>>(a, d);
+    if (f.nt == 64 && f.nv == 1) ln_bwd_k<T, 1, 64, 1, COLS, RES><<<g, 256, 0, st>>>(a, d);
+    else if (f.nt == 512) ln_bwd_k<T, 1, 512, 1, COLS, RES><<<g, 512, 0, st>>>(a, d);
     else if constexpr (COLS != SHORT) {
-        if (f.nt == 128) ln_bwd_k<T, 1, 128, 4, COLS><<<g, 512, 0, st>>>(a, d);
-        else if (f.nt == 256) ln_bwd_k<T, 1, 256, 2, COLS><<<g, 512, 0, st>>>(a, d);
-        else if (f.nv == 1) ln_bwd_k<T, 1, 1024, 1, COLS><<<g, 1024, 0, st>>>(a, d);
-        else if constexpr (sizeof(T) == 4) ln_bwd_k<T, 2, 1024, 1, COLS><<<g, 1024, 0, st>>>(a, d);
+        if (f.nt == 128) ln_bwd_k<T, 1, 128, 4, COLS, RES><<<g, 512, 0, st>>>(a, d);
+        else if (f.nt == 256) ln_bwd_k<T, 1, 256, 2, COLS, RES><<<g, 512, 0, st>>>(a, d);
+        else if (f.nv == 1) ln_bwd_k<T, 1, 1024, 1, COLS, RES><<<g, 1024, 0, st>>>(a, d);
+        else if constexpr (sizeof(T) == 4) ln_bwd_k<T, 2, 1024, 1, COLS, RES><<<g, 1024, 0, st>>>(a, d);
     }
 }
 static unsigned grid_y(long n) { return (unsigned)(n < 65535 ? n : 65535); }
@@ -856,7 +887,7 @@ static int ln_fwd(const char* what, NormArgs a, const Drop& d, bool res, int typ
         });
     });
 }
-static int ln_bwd(const char* what, NormArgs a, const Drop& d, int type, void* ws, size_t ws_bytes, hipStream_t st) {
+static int ln_bwd(const char* what, NormArgs a, const Drop& d, bool res, int type, void* ws, size_t ws_bytes, hipStream_t st) {
     if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, std::max(a.ldx, a.lddy), type, 1), ws, ws_bytes)) return rc;
     const Form f = ln_form(a.C, std::max(a.ldx, a.lddy), type, true);
     a.lg = f.lg;
@@ -868,7 +899,8 @@ static int ln_bwd(const char* what, NormArgs a, const Drop& d, int type, void* w
             if (f.nt) {
                 parts = ln_blocks(a.rows, f, true);
                 a.part = (float*)ws;
-                ln_bwd_launch<T, COLS>(a, d, f, (unsigned)parts, st);
+                if (res) ln_bwd_launch<T, COLS, true>(a, d, f, (unsigned)parts, st);
+                else ln_bwd_launch<T, COLS, false>(a, d, f, (unsigned)parts, st);
             } else if constexpr (COLS != SHORT) {
                 const SplitPlan sp = split_plan(a.C, sizeof(T));
                 Chunk* c = (Chunk*)ws;
@@ -920,7 +952,8 @@ extern "C" int siv_layer_norm_bwd(const void* dy, long lddy, const void* x, long
     a.x = x; a.dy = dy; a.weight = weight; a.dx = dx; a.dw = dweight; a.db = dbias; a.accumulate = accumulate;
     a.rows = rows; a.C = C; a.ldx = ldx; a.lddy = lddy; a.eps = eps; a.wf32 = wtype == SIV_F32;
     if (int rc = ln_check("layer_norm_bwd", a, type, wtype)) return rc;
-    return ln_bwd("layer_norm_bwd", a, make_drop(nullptr, 0, 0, nullptr, 0.f), type, ws, ws_bytes, (hipStream_t)stream);
+    return ln_bwd("layer_norm_bwd", a, make_drop(nullptr, 0, 0, nullptr, 0.f), false, type, ws, ws_bytes,
+                  (hipStream_t)stream);
 }
 extern "C" int siv_add_layer_norm_fwd(const void* x, const void* residual, const uint8_t* keep, uint64_t seed,
                                       uint64_t stream_id, const uint64_t* epoch, float p, const void* weight,
@@ -946,6 +979,6 @@ extern "C" int siv_add_layer_norm_bwd(const void* dy, const void* ds, const void
     a.accumulate = accumulate;
     a.rows = rows; a.C = C; a.ldx = C; a.lddy = C; a.eps = eps; a.wf32 = wtype == SIV_F32;
     if (int rc = ln_check("add_layer_norm_bwd", a, type, wtype)) return rc;
-    return ln_bwd("add_layer_norm_bwd", a, make_drop(keep, seed, stream_id, epoch, p), type, ws, ws_bytes,
+    return ln_bwd("add_layer_norm_bwd", a, make_drop(keep, seed, stream_id, epoch, p), true, type, ws, ws_bytes,
                   (hipStream_t)stream);
 }
