@@ -1,8 +1,8 @@
 // Dropout whose mask is never stored (fp32, bf16, fp16): out = [residual +] keep * act(x) / (1 - p).
 // Element i of a call is component i % 4 of Philox(i / 4, stream id, seed): forward and backward draw it again instead
 // of writing and reading a mask.  Bytes: one tensor read and one written (two read onto a residual).  Arithmetic: per
-// four elements 18 products of 32 x 32 bits and 36 three-way xors; with 16-bit elements that takes about as long as
-// the traffic (315 M elements of bf16: 241 us, of which 227 remain with the generator left out).
+// four elements 18 products of 32 x 32 bits and 18 three-way xors; with 16-bit elements that takes about as long as
+// the traffic.  315 M elements of bf16: 220 us = 5.7 TB/s (a device copy: 237-285 us); 78.6 M of fp32: 108 us = 5.8.
 #include "elem_types.h"
 
 namespace siv {
@@ -88,8 +88,8 @@ static void dropout_launch(int what, const T* in, const T* other, const Drop& d,
 // Packs per thread and grid.  fp32 is bound by HBM: one pack a thread and a block per tile (78.6 M elements: 107 us =
 // 5.9 TB/s; a grid of 4096 that walks the tensor 118, two packs 110).  Of 16-bit types a pack is two Philox calls, whose
 // arithmetic is as long as their traffic: several packs a thread, and for tensors that fill the chip many times over a
-// block per tile (315 M elements of bf16: 241 us with four packs, 256 with two, 258 with two and a grid of 2048), for
-// smaller ones a grid of 2048 (19.7 M: 13.8 us; block per tile 15.5 with two packs, 16.6 with four).
+// block per tile (315 M elements of bf16: 220-241 us with four packs, 256 with two, 258 with two and a grid of 2048), for
+// smaller ones a grid of 2048 (19.7 M: 14 us; block per tile 15.5 with two packs, 16.6 with four).  BIG lies between.
 constexpr long BLOCKS_MAX = 1L << 20, BIG = 1L << 27;
 template <typename T, bool AL>
 static void dropout_size(int what, const T* in, const T* other, const Drop& d, float slope, T* out, long n,

@@ -5,6 +5,14 @@
 // The mean is summed twice: m0 = sum x / C, then d = x - m0, delta = sum d / C, var = sum d^2 / C - delta^2.  x - m0
 // is exact or nearly so, and delta takes back the rounding of m0, so rows far off zero keep their deviations.
 // The backward pass forms the statistics again from the row it reads anyway, so forward leaves nothing behind.
+//
+// Bound by HBM: forward reads and writes the tensor once, backward reads two and writes one (residual form: two and two,
+// three and two).  What the kernels move is that: WRITE_SIZE of a 4915200 x 64 fp32 call (1.26 GB tensors) is the tensor
+// to 0.04 %.  Times below: back-to-back calls on one MI355X, TB/s of those bytes; a device copy of that size runs at
+// 4.5-5.2.  4915200 x 64 fp32: forward 441 us (5.7), backward 664 us (5.7); residual form 614400 x 128 fp32: 227 (5.5) and
+// 304 us (5.2).  With 16-bit elements the arithmetic of the backward pass (about 16 operations an element on a lane that
+// holds eight) is close behind: 614400 x 128 bf16 forward 56 us (5.6), backward 88 us (5.4); 100000 x 601, where 52 of 128
+// lanes have no column, 111 us (3.2).
 #include <algorithm>
 #include "elem_types.h"
 
@@ -227,7 +235,8 @@ __device__ __forceinline__ void pack_sums(const Span<T, COLS>& sp, bool ragged, 
 
 // residual + dropout(x) of one pack from element i on, as it is held
 template <typename T, int COLS>
-__device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res, const Drop& d, uint64_t sid, long i, int hi) {
+__device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res, const Drop& d, uint64_t sid, long i,
+                                            int hi) {
     constexpr int N = Pack<T>::N;
     Pack<T> s;
     if (d.mode == 0) {
@@ -244,9 +253,10 @@ __device__ __forceinline__ Pack<T> add_drop(const Pack<T>& x, const Pack<T>& res
 
 // ---- rows held in registers -----------------------------------------------------------------------------------------
 // A row is spread over 2^lg lanes of a wave, 64 >> lg rows to a wave and four waves to a block (NT = 64), or over NT
-// threads, R rows to a block; a lane holds NV packs of 16 bytes.  One pass over the data.  Blocks walk the rows in strides of
-// the grid, so that weights and the parameters' gradients stay in registers; the next row is requested before the
-// present one is worked on.
+// threads, R rows to a block; a lane holds NV packs of 16 bytes.  One pass over the data.  Blocks walk the rows in
+// strides of the grid, so that weights and the parameters' gradients stay in registers; the next row is requested before
+// the present one is worked on (not in the forward wave form, whose blocks take one step: 4915200 x 64 fp32 483 us with a
+// grid of 2048 that walks, 441 us with a block per step).
 template <typename T, int NV, int NT, int R, int COLS, bool RES>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
@@ -334,7 +344,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, 
 }
 
 // The same rows backward.  Each lane sums dy h and dy of its columns over the rows it sees; a block's sums go to
-// a.part, or straight to the results where there is one block.
+// a.part, or straight to the results where there is one block.  x and dy of the wave form, which nothing is expected to
+// read after this, are loaded non-temporally (4915200 x 64 fp32: 697 -> 668 us, 614400 x 128 bf16 104 -> 96).
 template <typename T, int NV, int NT, int R, int COLS, bool RES>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_bwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
@@ -739,7 +750,8 @@ __global__ __launch_bounds__(1024) void ln_param_sum_k(const float* __restrict__
     if (i < C2) {
         long k = down;
         for (; k + 3 * DOWN < parts; k += 4 * DOWN)          // four loads at a time
-            t += (part[k * C2 + i] + part[(k + DOWN) * C2 + i]) + (part[(k + 2 * DOWN) * C2 + i] + part[(k + 3 * DOWN) * C2 + i]);
+            t += (part[k * C2 + i] + part[(k + DOWN) * C2 + i]) +
+                 (part[(k + 2 * DOWN) * C2 + i] + part[(k + 3 * DOWN) * C2 + i]);
         for (; k < parts; k += DOWN) t += part[k * C2 + i];
     }
     sh[down][col] = t;
@@ -753,6 +765,12 @@ __global__ __launch_bounds__(1024) void ln_param_sum_k(const float* __restrict__
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
+// The forms, by packs of 16 bytes in a row (fp32: 4 elements, 16-bit: 8).  Up to 64: lanes of one wave.  Up to 128: forward
+// two packs to a lane (100000 x 601 bf16: 56 us, 64 with a pack to each of 128 threads), backward 128 threads, since two
+// packs' sums and gradients need 168 registers.  Then a thread per pack up to 1024, four, two or one rows to a block so
+// that a block's partial sums stand for several rows (20000 x 1024 bf16 backward: one row to a block 39 us, four 28).
+// Up to 2048: two packs a thread, except 16-bit backward, which spills.  Longer rows: chunks, whose second read costs half as
+// much again (300 x 100000 fp32: forward 63 us = 5.7 TB/s of three passes, backward 112 us = 5.4 of five).
 // Which kernel: a function of the row length and stride, the type and the direction alone, so that a row's result does
 // not depend on what is computed beside it.
 struct Form {
@@ -784,10 +802,15 @@ static Form ln_form(long C, long ld, int type, bool bwd) {
 static long ln_blocks(long rows, const Form& f, bool bwd) {
     const long steps = cdiv(rows, f.rows());
     if (!bwd) {
+        // (block forms walk: 2000 x 16384 bf16 28 us, with a block per row 35)
         const long cap = f.nt > 64 ? 2048 * 256L / f.threads() : f.nv == 2 ? 8192 : 1L << 20;
         return steps < cap ? steps : cap;
     }
     if (steps <= 4) return 1;                        // the parameters' gradients in one launch
+    // Blocks that stay: 768 x 256 threads in the wave form (4915200 x 64 fp32: 668 us; 512: 816, 640: 697, 896: 712,
+    // 1024: 704: too few bytes in flight below, more of them than HBM serves well above), 1024 x 256 with the barriers of
+    // the block forms (8192 x 4096 fp32: 92 us; 768: 112, 1280: 130).  Four steps each at least, where that leaves a block
+    // per CU.
     const long cap = (f.nt == 64 ? 768 : 1024) * 256L / f.threads();
     const long b = steps / 4 > 256 ? steps / 4 : 256;
     return std::min(std::min(b, cap), steps);
@@ -809,7 +832,8 @@ static size_t ln_ws_bytes(long rows, long C, long ld, int type, int bwd) {
     return blocks > 1 ? (size_t)blocks * 2 * C * 4 : 0;
 }
 static int ln_check(const char* what, const NormArgs& a, int type, int wtype) {
-    SIV_CHECK_ARG(a.rows > 0 && a.C > 0 && a.C < (1L << 31) && a.rows < (1L << 40), "%s: rows and C must be positive (C < 2^31)", what);
+    SIV_CHECK_ARG(a.rows > 0 && a.C > 0 && a.C < (1L << 31) && a.rows < (1L << 40),
+                  "%s: rows and C must be positive (C < 2^31)", what);
     SIV_CHECK_ARG(a.ldx >= a.C && a.lddy >= a.C, "%s: a row stride is shorter than the row", what);
     SIV_CHECK_ARG(known_type(type), "%s: unknown element type", what);
     SIV_CHECK_ARG(wtype == SIV_F32 || wtype == type, "%s: weights must be fp32 or of the activations' type", what);
@@ -861,7 +885,8 @@ static void ln_bwd_launch(const NormArgs& a, const Drop& d, const Form& f, unsig
 }
 static unsigned grid_y(long n) { return (unsigned)(n < 65535 ? n : 65535); }
 
-static int ln_fwd(const char* what, NormArgs a, const Drop& d, bool res, int type, void* ws, size_t ws_bytes, hipStream_t st) {
+static int ln_fwd(const char* what, NormArgs a, const Drop& d, bool res, int type, void* ws, size_t ws_bytes,
+                  hipStream_t st) {
     if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, a.ldx, type, 0), ws, ws_bytes)) return rc;
     const Form f = ln_form(a.C, a.ldx, type, false);
     a.lg = f.lg;
@@ -887,7 +912,8 @@ static int ln_fwd(const char* what, NormArgs a, const Drop& d, bool res, int typ
         });
     });
 }
-static int ln_bwd(const char* what, NormArgs a, const Drop& d, bool res, int type, void* ws, size_t ws_bytes, hipStream_t st) {
+static int ln_bwd(const char* what, NormArgs a, const Drop& d, bool res, int type, void* ws, size_t ws_bytes,
+                  hipStream_t st) {
     if (int rc = ln_check_ws(what, ln_ws_bytes(a.rows, a.C, std::max(a.ldx, a.lddy), type, 1), ws, ws_bytes)) return rc;
     const Form f = ln_form(a.C, std::max(a.ldx, a.lddy), type, true);
     a.lg = f.lg;
@@ -913,9 +939,14 @@ static int ln_bwd(const char* what, NormArgs a, const Drop& d, bool res, int typ
             }
             SIV_CHECK_LAUNCH(what);
             if ((a.dw || a.db) && parts > 1) {
-                if (parts <= 32) ln_param_sum_k<T, 4><<<(unsigned)cdiv(2 * a.C, 256), 1024, 0, st>>>(a.part, parts, a);
-                else if (parts <= 256 || a.C >= 4096) ln_param_sum_k<T, 16><<<(unsigned)cdiv(2 * a.C, 64), 1024, 0, st>>>(a.part, parts, a);
-                else ln_param_sum_k<T, 64><<<(unsigned)cdiv(2 * a.C, 16), 1024, 0, st>>>(a.part, parts, a);
+                // threads down a column: a few additions each, but enough blocks (768 x 128 sums: 4.9 us with 64; 21 x
+                // 200000: 8 us with 4, 31 with 64)
+                const float* p = a.part;
+                const int down = parts <= 32 ? 4 : parts <= 256 || a.C >= 4096 ? 16 : 64;
+                const unsigned g = (unsigned)cdiv(2 * a.C * down, 1024);
+                if (down == 4) ln_param_sum_k<T, 4><<<g, 1024, 0, st>>>(p, parts, a);
+                else if (down == 16) ln_param_sum_k<T, 16><<<g, 1024, 0, st>>>(p, parts, a);
+                else ln_param_sum_k<T, 64><<<g, 1024, 0, st>>>(p, parts, a);
                 SIV_CHECK_LAUNCH(what);
             }
             return SIV_OK;

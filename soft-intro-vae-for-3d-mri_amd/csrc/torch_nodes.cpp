@@ -246,7 +246,12 @@ struct AddLayerNormBackward : Node {
                 out[3] = g.out(g.db);
             }
         }
-        return first_order(std::move(out), sources, "add_layer_norm");
+        out = first_order(std::move(out), sources, "add_layer_norm");
+        if (!grads[0].defined()) {         // what is handed on as it came keeps its own history
+            if (need_r) out[1] = grads[1];
+            if (need_x && !mask.on) out[0] = grads[1];
+        }
+        return out;
     }
 };
 
@@ -280,8 +285,9 @@ struct DropoutBackward : Node {
                                  ptr(out[0]), type_code(g.scalar_type()), g.numel(), stream_of(g)),
                     "siv_dropout_bwd");
         }
-        if (need_r) out[1] = dy;
-        return first_order(std::move(out), sources, "dropout");
+        out = first_order(std::move(out), sources, "dropout");
+        if (need_r) out[1] = grads[0];     // handed on as it came, with its own history
+        return out;
     }
 };
 

@@ -643,7 +643,9 @@ def _first_order(what):
             sources = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad]
             if not sources:
                 return outs
-            return tuple(None if o is None else _NoSecondDerivative.apply(o, what, *sources) for o in outs)
+            # (an upstream gradient that is handed on as it came keeps its own history)
+            return tuple(o if o is None or any(o is g for g in grads) else _NoSecondDerivative.apply(o, what, *sources)
+                         for o in outs)
         return run
     return wrap
 

@@ -267,6 +267,12 @@ def test_refusals(hip):
         assert torch.equal(dx, first)
         with pytest.raises(RuntimeError, match="differentia"):
             torch.autograd.grad((dx * xg.sin()).sum(), xg)
+    # the residual's gradient is the upstream one, with its history
+    a, res = rnd(2, 4, 8).cuda().requires_grad_(), rnd(3, 4, 8).cuda().requires_grad_()
+    for f in (lambda: o.dropout(xg, key(), 0.5, residual=res), lambda: o.add_layer_norm(xg, res, keep=key(), p=0.5)[1],
+              lambda: o.add_layer_norm(xg, res)[1]):
+        dr, = torch.autograd.grad((f() * a).sum(), res, create_graph=True)
+        assert torch.equal(torch.autograd.grad(dr.square().sum(), a)[0], 2 * a.detach())
     dx, = torch.autograd.grad(o.dropout(xg, key(), 0.5).sum(), xg, create_graph=True)      # does not depend on xg
     assert torch.equal(torch.autograd.grad((dx * xg.sin()).sum(), xg)[0], dx.detach() * xg.detach().cos())
 
