@@ -807,8 +807,8 @@ static long ln_blocks(long rows, const Form& f, bool bwd) {
         return steps < cap ? steps : cap;
     }
     if (steps <= 4) return 1;                        // the parameters' gradients in one launch
-    // Blocks that stay: 768 x 256 threads in the wave form (4915200 x 64 fp32: 668 us; 512: 816, 640: 697, 896: 712,
-    // 1024: 704: too few bytes in flight below, more of them than HBM serves well above), 1024 x 256 with the barriers of
+    // Blocks that stay: 768 x 256 threads in the wave form (4915200 x 64 fp32: 664 us; 640: 697, 896: 712, 1024: 704;
+    // with plain loads and stores 768: 688, 512: 816, 1024: 738), 1024 x 256 with the barriers of
     // the block forms (8192 x 4096 fp32: 92 us; 768: 112, 1280: 130).  Four steps each at least, where that leaves a block
     // per CU.
     const long cap = (f.nt == 64 ? 768 : 1024) * 256L / f.threads();
@@ -940,7 +940,7 @@ static int ln_bwd(const char* what, NormArgs a, const Drop& d, bool res, int typ
             SIV_CHECK_LAUNCH(what);
             if ((a.dw || a.db) && parts > 1) {
                 // threads down a column: a few additions each, but enough blocks (768 x 128 sums: 4.9 us with 64; 21 x
-                // 200000: 8 us with 4, 31 with 64)
+                // 200000: 6 us with 4, 30 with 64)
                 const float* p = a.part;
                 const int down = parts <= 32 ? 4 : parts <= 256 || a.C >= 4096 ? 16 : 64;
                 const unsigned g = (unsigned)cdiv(2 * a.C * down, 1024);

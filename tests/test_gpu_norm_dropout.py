@@ -610,6 +610,35 @@ def test_another_stream_and_two_at_once():
             assert all(torch.equal(a, b) for a, b in zip(g, w))
 
 
+def test_recomputed_branch_and_inference_mode():
+    """Activation checkpointing (the branch runs again in backward, drawing the same masks), inference mode, and a second
+    Python thread give what the plain call gives."""
+    import threading
+    from torch.utils.checkpoint import checkpoint
+    o, p, shape = ops(), 0.25, (2, 64, 4, 5, 6)
+    x, ps, dy = branch_inputs(shape)
+    leaves = [t.detach().requires_grad_() for t in (x, *ps)]
+    out = branch(o, *leaves, key(1, 2), key(1, 3), p)
+    want = [out.detach()] + list(torch.autograd.grad(out, leaves, dy))
+    out = checkpoint(lambda *a: branch(o, *a, key(1, 2), key(1, 3), p), *leaves, use_reentrant=False)
+    got = [out.detach()] + list(torch.autograd.grad(out, leaves, dy))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        assert torch.equal(branch(o, x, *ps, key(1, 2), key(1, 3), p), want[0])
+    res = []
+
+    def work():
+        ls = [t.detach().requires_grad_() for t in (x, *ps)]
+        y = branch(o, *ls, key(1, 2), key(1, 3), p)
+        res.append([y.detach()] + list(torch.autograd.grad(y, ls, dy)))
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(res) == 2 and all(torch.equal(a, b) for r in res for a, b in zip(r, want))
+
+
 def test_captured_branches_replay(hip):
     """Two captured graphs of forward + backward, replayed with eager work between, each replay with the next epoch's
     masks, against the eager result of the same epoch."""
