@@ -808,9 +808,8 @@ static long ln_blocks(long rows, const Form& f, bool bwd) {
     }
     if (steps <= 4) return 1;                        // the parameters' gradients in one launch
     // Blocks that stay: 768 x 256 threads in the wave form (4915200 x 64 fp32: 664 us; 640: 697, 896: 712, 1024: 704;
-    // with plain loads and stores 768: 688, 512: 816, 1024: 738), 1024 x 256 with the barriers of
-    // the block forms (8192 x 4096 fp32: 92 us; 768: 112, 1280: 130).  Four steps each at least, where that leaves a block
-    // per CU.
+    // with plain loads and stores 768: 688, 512: 816, 1024: 738), 1024 x 256 with the barriers of the block forms (8192 x
+    // 4096 fp32: 92 us; 768: 112, 1280: 130).  Four steps each at least, where that leaves a block per CU.
     const long cap = (f.nt == 64 ? 768 : 1024) * 256L / f.threads();
     const long b = steps / 4 > 256 ? steps / 4 : 256;
     return std::min(std::min(b, cap), steps);

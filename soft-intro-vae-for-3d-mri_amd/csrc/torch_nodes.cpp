@@ -382,12 +382,13 @@ bool dropout(const Tensor& x, const Tensor& res, const Mask& m, double slope, Te
 }
 
 // ---- Python ------------------------------------------------------------------------------------------------------------
-// a tensor of exactly torch's own types, or None (undefined); anything else: not for here
+// a tensor of exactly torch's own types, or None (undefined); anything else: not for here.  Nor a tensor with a forward-mode
+// tangent, which the nodes would lose (the Python functions refuse it).
 bool tensor_arg(PyObject* o, Tensor& t) {
     if (o == Py_None) return true;
     if (!THPVariable_CheckExact(o)) return false;
     t = THPVariable_Unpack(o);
-    return true;
+    return !t._fw_grad(0).defined();
 }
 bool float_arg(PyObject* o, double& v) {
     v = PyFloat_AsDouble(o);

@@ -639,6 +639,23 @@ def test_recomputed_branch_and_inference_mode():
     assert len(res) == 2 and all(torch.equal(a, b) for r in res for a, b in zip(r, want))
 
 
+def test_forward_mode_derivatives_are_refused(hip):
+    """A tensor with a tangent: there is no forward-mode rule, and none may be lost without a word."""
+    import torch.autograd.forward_ad as fwd
+    o, gen = ops(), torch.Generator(device="cuda").manual_seed(3)
+    x, r, t = (torch.randn(6, 40, device="cuda", generator=gen) for _ in range(3))
+    w, tw = (torch.randn(40, device="cuda", generator=gen) for _ in range(2))
+    with fwd.dual_level():
+        dx, dw = fwd.make_dual(x, t), fwd.make_dual(w, tw)
+        for call in (lambda: o.layer_norm(dx, w), lambda: o.layer_norm(x, dw), lambda: o.layer_norm(x, w, dw),
+                     lambda: o.dropout(dx, key(1, 2), 0.5), lambda: o.dropout(x, key(1, 2), 0.5, residual=dx),
+                     lambda: o.add_layer_norm(dx, r, w), lambda: o.add_layer_norm(r, dx, w),
+                     lambda: o.add_layer_norm(x, r, dw)):
+            with pytest.raises(RuntimeError):
+                call()
+        assert torch.equal(o.layer_norm(x, w), o.layer_norm(x.clone(), w))        # without a tangent: as ever
+
+
 def test_captured_branches_replay(hip):
     """Two captured graphs of forward + backward, replayed with eager work between, each replay with the next epoch's
     masks, against the eager result of the same epoch."""
