@@ -3,12 +3,13 @@
 // A training call on a small tensor is host time: the same operators as Python autograd functions spend most of it in
 // interpreted code on autograd's own thread (a layer norm of 8 x 1200 and its gradients: 107 us, and 59 us for a native
 // operator of torch).  The functions here take the common case -- plain dense device tensors (or slices of wider
-// rows) on the current device, arguments in range -- and return None for everything else; the caller then takes the
-// Python path, which knows every layout and words every refusal.  Both call the same entry points of libsiv, whose
+// rows) on the current device, arguments in range, no trace being recorded -- and return None for everything else; the
+// caller then takes the Python path, which knows every layout and words every refusal.  Both call the same entry points of libsiv, whose
 // addresses are handed in by `bind`, so that whichever build of the library is loaded is the one that runs.
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -382,6 +383,9 @@ bool dropout(const Tensor& x, const Tensor& res, const Mask& m, double slope, Te
 }
 
 // ---- Python ------------------------------------------------------------------------------------------------------------
+// Whether a trace (torch.jit.trace) is being recorded.  It would see the allocations made here and not the kernels that fill
+// them, and replay uninitialised memory; of a Python function it records the call.
+bool recording() { return at::tracer::impl::is_dispatch_enabled(); }
 // a tensor of exactly torch's own types, or None (undefined); anything else: not for here.  Nor a tensor with a forward-mode
 // tangent, which the nodes would lose (the Python functions refuse it).
 bool tensor_arg(PyObject* o, Tensor& t) {
@@ -425,6 +429,7 @@ bool mask_args(PyObject* const* a, Mask& m) {
 PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     SIV_ARGS(6)
+    if (recording()) Py_RETURN_NONE;
     Tensor x, w, b, w_buf, b_buf, y;
     double eps;
     if (!tensor_arg(a[0], x) || !tensor_arg(a[1], w) || !tensor_arg(a[2], b) || !float_arg(a[3], eps) ||
@@ -442,6 +447,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_add_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     SIV_ARGS(12)
+    if (recording()) Py_RETURN_NONE;
     Tensor x, res, w, b, w_buf, b_buf, y, s;
     double eps;
     Mask m;
@@ -464,6 +470,7 @@ PyObject* py_add_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     SIV_ARGS(8)
+    if (recording()) Py_RETURN_NONE;
     Tensor x, res, out;
     double slope;
     Mask m;

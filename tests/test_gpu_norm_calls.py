@@ -1,0 +1,63 @@
+"""Layer norm, dropout and the residual step called through what torch puts around an operator: a recorded trace."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+CL3D = torch.channels_last_3d
+
+
+@pytest.fixture(params=["nodes", "python"])
+def hip(request):
+    """The backend, with its native autograd nodes and with the Python autograd functions only."""
+    import siv.backend as sb
+    sb.set_backend(None)
+    b = sb.get_backend()
+    nodes = b.nodes
+    assert nodes is not None, "siv/_siv_torch.so is not built"
+    if request.param == "python":
+        b.nodes = None
+    yield b
+    b.nodes = nodes
+
+
+def key(seed=5, sid=11):
+    from siv import rng
+    return rng.PhiloxKeep(seed, sid)
+
+
+def rnd(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def operators(o):
+    """(name, call on (x, residual, weight, bias)) of every entry point; one result each."""
+    return [("layer_norm", lambda x, r, w, b: o.layer_norm(x, w, b)),
+            ("layer_norm_plain", lambda x, r, w, b: o.layer_norm(x)),
+            ("dropout", lambda x, r, w, b: o.dropout(x, key(), 0.5)),
+            ("dropout_residual", lambda x, r, w, b: o.dropout(x, key(), 0.5, residual=r)),
+            ("act_dropout", lambda x, r, w, b: o.act_dropout(x, 0.2, key(), 0.5)),
+            ("add_layer_norm", lambda x, r, w, b: o.add_layer_norm(x, r, w, b, keep=key(), p=0.5)[0]),
+            ("add_layer_norm_sum", lambda x, r, w, b: o.add_layer_norm(x, r, w, b, keep=key(), p=0.5)[1]),
+            ("add_layer_norm_plain", lambda x, r, w, b: sum(o.add_layer_norm(x, r)))]
+
+
+NAMES = [n for n, _ in operators(None)]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_traced_calls_compute(hip, name, grad):
+    """A function recorded by torch.jit.trace computes the operator on the inputs of each later call (memory of other
+    values handed back to the allocator in between)."""
+    from siv import ops as o
+    f = dict(operators(o))[name]
+    args = [rnd(1, 6, 40), rnd(2, 6, 40), rnd(3, 40), rnd(4, 40)]
+    if grad:
+        args = [t.requires_grad_() for t in args]
+    traced = torch.jit.trace(lambda x, r, w, b: f(x, r, w, b) * 1.0 + 0 * (x + r + w + b), args, check_trace=False)
+    for seed in (10, 20, 30):
+        args = [rnd(seed + i, 6, 40) for i in range(2)] + [rnd(seed + i, 40) for i in (2, 3)]
+        want = f(*args)
+        junk = [torch.full((6, 40), 1e3, device="cuda") for _ in range(16)]
+        del junk
+        assert torch.equal(traced(*args), want)
