@@ -52,6 +52,11 @@ at::MemoryFormat format_of(const Tensor& t) {
 }
 bool dense(const Tensor& t) { return t.is_contiguous(format_of(t)); }
 Tensor made_dense(const Tensor& t) { return t.contiguous(format_of(t)); }
+// a saved tensor as it comes back: hooks (torch.autograd.graph.save_on_cpu and the like) keep values, not strides
+Tensor unpacked(const SavedVariable& v, std::shared_ptr<Node> saved_for = nullptr) {
+    Tensor t = v.unpack(std::move(saved_for));
+    return t.defined() && !dense(t) ? made_dense(t) : t;
+}
 Tensor empty_like_dense(const Tensor& t) { return at::empty(t.sizes(), t.options(), format_of(t)); }
 bool same_kind(const Tensor& a, const Tensor& x) {
     return a.scalar_type() == x.scalar_type() && a.device() == x.device() && a.sizes() == x.sizes() && dense(a);
@@ -169,7 +174,7 @@ struct LayerNormBackward : Node {
         Tensor dy = grads[0];
         if (!dy.defined() || !(need_x || need_w || need_b)) return out;
         {
-            Tensor x = x_.unpack(), w = w_.unpack();
+            Tensor x = x_.unpack(), w = unpacked(w_);       // (rows of x may lie apart)
             sources.insert(sources.end(), {x, w});
             at::AutoDispatchBelowADInplaceOrView guard;
             const c10::DeviceGuard device(x.device());
@@ -212,13 +217,12 @@ struct AddLayerNormBackward : Node {
         Tensor dy = grads[0], ds = grads[1];
         if (!(dy.defined() || ds.defined()) || !(need_x || need_r || need_w || need_b)) return out;
         {
-            Tensor s = s_.unpack(shared_from_this()), w = w_.unpack(), keep = keep_.unpack();
+            Tensor s = unpacked(s_, shared_from_this()), w = unpacked(w_), keep = unpacked(keep_);
             sources.insert(sources.end(), {s, w});
             at::AutoDispatchBelowADInplaceOrView guard;
             const c10::DeviceGuard device(s.device());
             const Rows r = rows_of(s);
             const int type = type_code(s.scalar_type());
-            if (!dense(s)) s = made_dense(s);
             if (ds.defined() && !dense(ds)) ds = made_dense(ds);
             Mask m = mask;
             m.keep = keep;
@@ -273,12 +277,11 @@ struct DropoutBackward : Node {
         Tensor dy = grads[0];
         if (!dy.defined()) return out;
         if (need_x) {
-            Tensor x = x_.unpack(), keep = keep_.unpack();
+            Tensor x = unpacked(x_), keep = unpacked(keep_);
             sources.push_back(x);
             at::AutoDispatchBelowADInplaceOrView guard;
             const c10::DeviceGuard device(dy.device());
             Tensor g = dense(dy) ? dy : made_dense(dy);
-            if (x.defined() && !dense(x)) x = made_dense(x);
             Mask m = mask;
             m.keep = keep;
             out[0] = empty_like_dense(g);

@@ -61,3 +61,38 @@ def test_traced_calls_compute(hip, name, grad):
         junk = [torch.full((6, 40), 1e3, device="cuda") for _ in range(16)]
         del junk
         assert torch.equal(traced(*args), want)
+
+
+def volume(seed, dtype=torch.float32):
+    return rnd(seed, 2, 6, 3, 4, 5, dtype=dtype).contiguous(memory_format=CL3D)
+
+
+def masked_operators(o, m):
+    """Every entry point on volumes with the stored mask ``m`` where it takes one."""
+    return [lambda x, r, w, b: o.layer_norm(x, w, b), lambda x, r, w, b: o.dropout(x, m, 0.5),
+            lambda x, r, w, b: o.dropout(x, m, 0.5, residual=r), lambda x, r, w, b: o.act_dropout(x, 0.2, m, 0.5),
+            lambda x, r, w, b: o.act_dropout(x, 0.2, key(), 0.5),
+            lambda x, r, w, b: sum(o.add_layer_norm(x, r, w, b, keep=m, p=0.5)),
+            lambda x, r, w, b: o.add_layer_norm(x, r, w, b, keep=m, p=0.5)[1]]
+
+
+@pytest.mark.parametrize("i", range(7))
+def test_saved_tensors_come_back_in_other_memory(hip, i):
+    """Hooks on saved tensors hand back the values in memory of another order (pinned host copies do): same gradients."""
+    from siv import ops as o
+    m = (volume(9) > 0).to(torch.uint8)
+    f = masked_operators(o, m)[i]
+    args = [t.requires_grad_() for t in (volume(1), volume(2), rnd(3, 6), rnd(4, 6))]
+    dy = volume(5)
+
+    def apart(t):
+        if t.dim() == 5:
+            return t.contiguous()                                   # NCDHW memory
+        return torch.stack((t, t + 1), -1)[..., 0] if t.dim() == 1 else t
+    want = torch.autograd.grad(f(*args), args, dy, allow_unused=True)
+    for hooks in (torch.autograd.graph.saved_tensors_hooks(lambda t: t, apart),
+                  torch.autograd.graph.save_on_cpu(pin_memory=True), torch.autograd.graph.save_on_cpu()):
+        with hooks:
+            y = f(*args)
+        got = torch.autograd.grad(y, args, dy, allow_unused=True)
+        assert all(a is b or torch.equal(a, b) for a, b in zip(got, want))
