@@ -52,17 +52,24 @@ at::MemoryFormat format_of(const Tensor& t) {
 }
 bool dense(const Tensor& t) { return t.is_contiguous(format_of(t)); }
 Tensor made_dense(const Tensor& t) { return t.contiguous(format_of(t)); }
-// a saved tensor as it comes back: hooks (torch.autograd.graph.save_on_cpu and the like) keep values, not strides
-Tensor unpacked(const SavedVariable& v, std::shared_ptr<Node> saved_for = nullptr) {
-    Tensor t = v.unpack(std::move(saved_for));
-    return t.defined() && !dense(t) ? made_dense(t) : t;
-}
 Tensor empty_like_dense(const Tensor& t) { return at::empty(t.sizes(), t.options(), format_of(t)); }
 bool same_kind(const Tensor& a, const Tensor& x) {
     return a.scalar_type() == x.scalar_type() && a.device() == x.device() && a.sizes() == x.sizes() && dense(a);
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+// A saved tensor as it comes back.  Hooks (torch.autograd.graph.save_on_cpu and the like) keep values, not strides, and may
+// hand back anything: the kernels take no other type, sizes or device than those that were saved.
+Tensor unpacked(const SavedVariable& v, at::ScalarType type, at::IntArrayRef sizes, at::Device device,
+                std::shared_ptr<Node> saved_for = nullptr, bool any_rows = false) {
+    Tensor t = v.unpack(std::move(saved_for));
+    if (!t.defined()) return t;
+    TORCH_CHECK(t.scalar_type() == type && t.sizes() == sizes && t.device() == device && t.layout() == at::kStrided,
+                "a saved tensor came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), " where ", type, " ", sizes,
+                " on ", device, " was saved");
+    return any_rows || dense(t) ? t : made_dense(t);
+}
 
 struct Rows {
     int64_t rows, C;
@@ -174,7 +181,8 @@ struct LayerNormBackward : Node {
         Tensor dy = grads[0];
         if (!dy.defined() || !(need_x || need_w || need_b)) return out;
         {
-            Tensor x = x_.unpack(), w = unpacked(w_);       // (rows of x may lie apart)
+            Tensor x = unpacked(x_, dy.scalar_type(), dy.sizes(), dy.device(), nullptr, true),
+                   w = unpacked(w_, ptype, {rows_of(dy).C}, dy.device());
             sources.insert(sources.end(), {x, w});
             at::AutoDispatchBelowADInplaceOrView guard;
             const c10::DeviceGuard device(x.device());
@@ -217,7 +225,10 @@ struct AddLayerNormBackward : Node {
         Tensor dy = grads[0], ds = grads[1];
         if (!(dy.defined() || ds.defined()) || !(need_x || need_r || need_w || need_b)) return out;
         {
-            Tensor s = unpacked(s_, shared_from_this()), w = unpacked(w_), keep = unpacked(keep_);
+            const Tensor& up = dy.defined() ? dy : ds;
+            Tensor s = unpacked(s_, up.scalar_type(), up.sizes(), up.device(), shared_from_this()),
+                   w = unpacked(w_, ptype, {rows_of(up).C}, up.device()),
+                   keep = unpacked(keep_, at::kByte, up.sizes(), up.device());
             sources.insert(sources.end(), {s, w});
             at::AutoDispatchBelowADInplaceOrView guard;
             const c10::DeviceGuard device(s.device());
@@ -277,7 +288,8 @@ struct DropoutBackward : Node {
         Tensor dy = grads[0];
         if (!dy.defined()) return out;
         if (need_x) {
-            Tensor x = unpacked(x_), keep = unpacked(keep_);
+            Tensor x = unpacked(x_, dy.scalar_type(), dy.sizes(), dy.device()),
+                   keep = unpacked(keep_, at::kByte, dy.sizes(), dy.device());
             sources.push_back(x);
             at::AutoDispatchBelowADInplaceOrView guard;
             const c10::DeviceGuard device(dy.device());

@@ -832,6 +832,8 @@ class HipBackend:
         wt, weight, _ = self._affine("layer_norm backward", x, C, weight, None)
         if weight is None:
             wt = self._TYPES[pdtype]
+        elif (want_w or want_b) and weight.dtype != pdtype:
+            raise _lib.SivError(f"layer_norm backward: weights of {weight.dtype} for gradients of {pdtype}")
         dw, db, acc = self._affine_targets(x, C, pdtype, want_w, want_b, dw_out, db_out)
         dx = like(x) if want_x else None
         if rows == 0:
@@ -869,6 +871,8 @@ class HipBackend:
         wt, weight, _ = self._affine("add_layer_norm backward", s, C, weight, None)
         if weight is None:
             wt = self._TYPES[pdtype]
+        elif (want_w or want_b) and weight.dtype != pdtype:
+            raise _lib.SivError(f"add_layer_norm backward: weights of {weight.dtype} for gradients of {pdtype}")
         drop, held = self._drop_args("add_layer_norm backward", s, keep, p)
         dw, db, acc = self._affine_targets(s, C, pdtype, want_w, want_b, dw_out, db_out)
         dy, s = cl(dy), cl(s)

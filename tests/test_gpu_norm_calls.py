@@ -96,3 +96,39 @@ def test_saved_tensors_come_back_in_other_memory(hip, i):
             y = f(*args)
         got = torch.autograd.grad(y, args, dy, allow_unused=True)
         assert all(a is b or torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("i", [0, 1, 2, 4, 5, 6])
+def test_saved_tensors_that_come_back_changed_are_refused(hip, i):
+    """Hooks that hand back another device, type or shape than was saved -- of everything, of the weights, of the mask --
+    meet an error before anything is launched."""
+    from siv import ops as o
+    m = (volume(9) > 0).to(torch.uint8)
+    f = masked_operators(o, m)[i]
+    args = [t.requires_grad_() for t in (volume(1), volume(2), rnd(3, 6), rnd(4, 6))]
+    which = {"all": lambda t: True, "weight": lambda t: t.dim() == 1, "mask": lambda t: t.dtype == torch.uint8}
+    touched = {"weight": i in (0, 5, 6), "mask": i in (1, 2, 5, 6), "all": True}
+    for name, mine in which.items():
+        for change in (lambda t: t.cpu(), lambda t: t.to(torch.float16 if t.is_floating_point() else torch.int16),
+                       lambda t: t[:1], lambda t: t.double()):
+            if not touched[name]:
+                continue
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if mine(t) else t):
+                y = f(*args)
+            if name == "weight" and i == 6 and hip.nodes is None:
+                continue                    # (the sum alone: the Python function does not look at the weights)
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(y, args, volume(5), allow_unused=True)
+
+
+@pytest.mark.parametrize("held,back", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_weights_that_come_back_in_the_other_type_are_refused(hip, held, back):
+    """Weights may be float32 or of x's type; their gradient has the type they had, not the one a hook made of it."""
+    from siv import ops as o
+    x = rnd(1, 4, 40, dtype=torch.bfloat16).requires_grad_()
+    w = rnd(2, 40, dtype=held).requires_grad_()
+    for f in (lambda: o.layer_norm(x, w), lambda: o.add_layer_norm(x, x.detach(), w)[0]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.to(back) if t.dim() == 1 else t):
+            y = f()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, (x, w), rnd(3, 4, 40, dtype=torch.bfloat16))
