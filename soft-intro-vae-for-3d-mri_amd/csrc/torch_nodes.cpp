@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -398,9 +399,10 @@ bool dropout(const Tensor& x, const Tensor& res, const Mask& m, double slope, Te
 }
 
 // ---- Python ------------------------------------------------------------------------------------------------------------
-// Whether a trace (torch.jit.trace) is being recorded.  It would see the allocations made here and not the kernels that fill
-// them, and replay uninitialised memory; of a Python function it records the call.
-bool recording() { return at::tracer::impl::is_dispatch_enabled(); }
+// Whether calls are being recorded (torch.jit.trace) or watched (a dispatch mode, make_fx's among them).  A trace would see
+// the allocations made here and not the kernels that fill them, and replay uninitialised memory; of a Python function
+// torch.jit.trace records the call, and make_fx is refused there.
+bool recording() { return at::tracer::impl::is_dispatch_enabled() || c10::impl::dispatch_mode_enabled(); }
 // a tensor of exactly torch's own types, or None (undefined); anything else: not for here.  Nor a tensor with a forward-mode
 // tangent, which the nodes would lose (the Python functions refuse it).
 bool tensor_arg(PyObject* o, Tensor& t) {

@@ -689,6 +689,10 @@ class HipBackend:
 
     def _act_type(self, what, x, *others):
         """Type code of the activation tensor ``x``; every other tensor has to match its type, device and shape."""
+        if torch._C._len_torch_dispatch_stack():
+            from torch.fx.experimental.proxy_tensor import get_proxy_mode
+            if get_proxy_mode() is not None:        # the graph would hold the allocations and not the kernel
+                raise _lib.SivError(f"{what}: make_fx cannot record libsiv kernels")
         dt = x.dtype
         t = self._TYPES.get(dt)
         if t is None:

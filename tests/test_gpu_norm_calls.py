@@ -63,6 +63,23 @@ def test_traced_calls_compute(hip, name, grad):
         assert torch.equal(traced(*args), want)
 
 
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+@pytest.mark.parametrize("name", NAMES)
+def test_make_fx_is_refused(hip, name, mode):
+    """make_fx has no way to record a kernel: an error, not a graph without it.  Modes that only watch change nothing."""
+    from siv import ops as o
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    f = dict(operators(o))[name]
+    args = [rnd(1, 6, 40), rnd(2, 6, 40), rnd(3, 40), rnd(4, 40)]
+    with pytest.raises(Exception, match="make_fx"):
+        make_fx(f, tracing_mode=mode)(*args)
+    want = f(*args)
+    with FlopCounterMode(display=False):
+        got = f(*args)
+    assert torch.equal(got, want)
+
+
 def volume(seed, dtype=torch.float32):
     return rnd(seed, 2, 6, 3, 4, 5, dtype=dtype).contiguous(memory_format=CL3D)
 
