@@ -48,6 +48,16 @@ int type_code(at::ScalarType t) {
 bool on_current_device(const Tensor& t) {
     return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == c10::hip::current_device();
 }
+// torch.func's wrappers (vmap, grad, functionalize) and batched gradients: tensors without memory of their own
+bool wrapped(const Tensor& t) {
+    constexpr c10::DispatchKeySet keys({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched,
+                                        c10::DispatchKey::Functionalize, c10::DispatchKey::Batched});
+    return t.defined() && t.key_set().has_any(keys);
+}
+void require_plain(const variable_list& grads, const char* what) {
+    for (const Tensor& g : grads)
+        TORCH_CHECK(!wrapped(g), "the backward pass of ", what, " takes no batched or transformed gradients (torch.func, vmap)");
+}
 at::MemoryFormat format_of(const Tensor& t) {
     return t.dim() == 5 ? at::MemoryFormat::ChannelsLast3d : at::MemoryFormat::Contiguous;
 }
@@ -175,6 +185,7 @@ struct LayerNormBackward : Node {
         w_.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
+        require_plain(grads, "layer_norm");
         std::lock_guard<std::mutex> lock(mutex_);
         const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1),
                    need_b = task_should_compute_output(2);
@@ -225,6 +236,7 @@ struct AddLayerNormBackward : Node {
         variable_list out(4), sources = {grads[0], grads[1]};
         Tensor dy = grads[0], ds = grads[1];
         if (!(dy.defined() || ds.defined()) || !(need_x || need_r || need_w || need_b)) return out;
+        if (dy.defined() || (need_x && mask.on)) require_plain(grads, "add_layer_norm");       // (else ds is handed on)
         {
             const Tensor& up = dy.defined() ? dy : ds;
             Tensor s = unpacked(s_, up.scalar_type(), up.sizes(), up.device(), shared_from_this()),
@@ -289,6 +301,7 @@ struct DropoutBackward : Node {
         Tensor dy = grads[0];
         if (!dy.defined()) return out;
         if (need_x) {
+            require_plain(grads, "dropout");
             Tensor x = unpacked(x_, dy.scalar_type(), dy.sizes(), dy.device()),
                    keep = unpacked(keep_, at::kByte, dy.sizes(), dy.device());
             sources.push_back(x);
@@ -327,6 +340,7 @@ bool layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps, c
     {
         at::AutoDispatchBelowADInplaceOrView guard;
         y = empty_like_dense(x);
+        if (wrapped(y)) return false;      // (inside torch.func.grad what is allocated is wrapped too)
         const Scratch ws(r, type, 0, x);
         if (lib.norm_fwd(ptr(x), ld, ptr(w), ptr(b), wtype, (float)eps, ptr(y), type, r.rows, r.C, ptr(ws.t), ws.bytes,
                          stream_of(x)))
@@ -355,6 +369,7 @@ bool add_layer_norm(const Tensor& x, const Tensor& res, const Tensor& w, const T
         at::AutoDispatchBelowADInplaceOrView guard;
         y = empty_like_dense(x);
         s = empty_like_dense(x);
+        if (wrapped(y)) return false;
         const Scratch ws(r, type, 0, x);
         if (lib.add_fwd(ptr(x), ptr(res), m.stored(), m.seed, m.sid, m.epoch_ptr(), m.on ? m.p : 0.f, ptr(w), ptr(b), wtype,
                         (float)eps, ptr(s), ptr(y), type, r.rows, r.C, ptr(ws.t), ws.bytes, stream_of(x)))
@@ -381,6 +396,7 @@ bool dropout(const Tensor& x, const Tensor& res, const Mask& m, double slope, Te
     {
         at::AutoDispatchBelowADInplaceOrView guard;
         out = empty_like_dense(x);
+        if (wrapped(out)) return false;
         if (lib.drop_fwd(ptr(x), ptr(res), m.stored(), m.seed, m.sid, m.epoch_ptr(), m.on ? m.p : 0.f, (float)slope, ptr(out),
                          type_code(x.scalar_type()), x.numel(), stream_of(x)))
             return false;
@@ -403,13 +419,13 @@ bool dropout(const Tensor& x, const Tensor& res, const Mask& m, double slope, Te
 // the allocations made here and not the kernels that fill them, and replay uninitialised memory; of a Python function
 // torch.jit.trace records the call, and make_fx is refused there.
 bool recording() { return at::tracer::impl::is_dispatch_enabled() || c10::impl::dispatch_mode_enabled(); }
-// a tensor of exactly torch's own types, or None (undefined); anything else: not for here.  Nor a tensor with a forward-mode
-// tangent, which the nodes would lose (the Python functions refuse it).
+// a tensor of exactly torch's own types, or None (undefined); anything else: not for here.  Nor torch.func's wrappers, nor a
+// tensor with a forward-mode tangent, which the nodes would lose (the Python functions refuse both).
 bool tensor_arg(PyObject* o, Tensor& t) {
     if (o == Py_None) return true;
     if (!THPVariable_CheckExact(o)) return false;
     t = THPVariable_Unpack(o);
-    return !t._fw_grad(0).defined();
+    return !wrapped(t) && !t._fw_grad(0).defined();
 }
 bool float_arg(PyObject* o, double& v) {
     v = PyFloat_AsDouble(o);

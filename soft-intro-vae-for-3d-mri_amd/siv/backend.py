@@ -693,6 +693,10 @@ class HipBackend:
             from torch.fx.experimental.proxy_tensor import get_proxy_mode
             if get_proxy_mode() is not None:        # the graph would hold the allocations and not the kernel
                 raise _lib.SivError(f"{what}: make_fx cannot record libsiv kernels")
+        F = torch._C._functorch
+        for o in (x, *others):
+            if o is not None and (F.is_functorch_wrapped_tensor(o) or F.is_legacy_batchedtensor(o)):
+                raise _lib.SivError(f"{what}: takes no batched or transformed tensors (torch.func, vmap)")
         dt = x.dtype
         t = self._TYPES.get(dt)
         if t is None:

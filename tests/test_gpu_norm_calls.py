@@ -80,6 +80,29 @@ def test_make_fx_is_refused(hip, name, mode):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("name", NAMES)
+def test_function_transforms_are_refused(hip, name):
+    """vmap, grad, jvp, functionalize and batched gradients have no rule here: an error in words, not one about storage."""
+    import torch.func as F
+    from siv import ops as o
+    f = dict(operators(o))[name]
+    x, r, w, b = args = [rnd(1, 6, 40), rnd(2, 6, 40), rnd(3, 40), rnd(4, 40)]
+    calls = [lambda: F.vmap(lambda t: f(t, r, w, b))(torch.stack((x, x))), lambda: F.grad(lambda t: f(t, r, w, b).sum())(x),
+             lambda: F.grad(lambda t: (t * f(*args)).sum())(x), lambda: F.jvp(lambda t: f(t, r, w, b), (x,), (x,)),
+             lambda: F.functionalize(lambda t: f(t, r, w, b))(x)]
+    xg = x.clone().requires_grad_()
+    y = f(xg, r, w, b)
+    calls.append(lambda: torch.autograd.grad(y, xg, rnd(5, 3, 6, 40), is_grads_batched=True))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="functorch transforms|torch.func"):
+            call()
+    assert torch.equal(f(*args), y)
+    # what is handed on as it came may be anything
+    rg, up = r.clone().requires_grad_(), rnd(5, 3, 6, 40)
+    for out in (o.dropout(x, key(), 0.5, residual=rg), o.add_layer_norm(x, rg, keep=key(), p=0.5)[1]):
+        assert torch.equal(torch.autograd.grad(out, rg, up, is_grads_batched=True)[0], up)
+
+
 def volume(seed, dtype=torch.float32):
     return rnd(seed, 2, 6, 3, 4, 5, dtype=dtype).contiguous(memory_format=CL3D)
 
