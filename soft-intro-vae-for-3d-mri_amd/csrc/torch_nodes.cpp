@@ -161,7 +161,9 @@ struct AffineGrads {
     int accumulate = 0;
     AffineGrads(bool need_w, bool need_b, const Tensor& w_buf, const Tensor& b_buf, at::ScalarType type, int64_t C,
                 const Tensor& like) {
-        const bool direct = (need_w || need_b) && (!need_w || w_buf.defined()) && (!need_b || b_buf.defined());
+        // (one parameter as weight and bias: its buffer would be added into from two places at once)
+        const bool direct = (need_w || need_b) && (!need_w || w_buf.defined()) && (!need_b || b_buf.defined()) &&
+                            !(need_w && need_b && w_buf.data_ptr() == b_buf.data_ptr());
         accumulate = direct;
         if (need_w) dw = direct ? w_buf : at::empty({C}, like.options().dtype(type));
         if (need_b) db = direct ? b_buf : at::empty({C}, like.options().dtype(type));

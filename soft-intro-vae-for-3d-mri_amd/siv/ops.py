@@ -737,6 +737,8 @@ def _affine_bufs(bufs, need_w, need_b):
     w_buf, b_buf = bufs
     if (need_w and w_buf is None) or (need_b and b_buf is None):
         return None, None
+    if need_w and need_b and w_buf.data_ptr() == b_buf.data_ptr():
+        return None, None       # one parameter as weight and bias: it would be added into from two places at once
     return (w_buf if need_w else None), (b_buf if need_b else None)
 
 

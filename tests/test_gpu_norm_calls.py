@@ -172,3 +172,21 @@ def test_weights_that_come_back_in_the_other_type_are_refused(hip, held, back):
             y = f()
         with pytest.raises(RuntimeError):
             torch.autograd.grad(y, (x, w), rnd(3, 4, 40, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("R,C", [(5, 96), (9603, 256), (300, 9001)])
+def test_one_parameter_as_weight_and_bias(hip, R, C):
+    """Both gradients of a parameter that is weight and bias at once reach its flat optimiser buffer: the sum of the two."""
+    from siv import ops as o
+    from siv.optim import FlatAdam
+    x, dy = rnd(1, R, C), rnd(2, R, C)
+    w = torch.nn.Parameter(1 + 0.2 * rnd(3, C))
+    a, b = w.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    dw, db = torch.autograd.grad(o.layer_norm(x, a, b), (a, b), dy)
+    opt = FlatAdam([w], lr=1e-3)
+    opt.zero_grad()
+    o.layer_norm(x, w, w).backward(dy)
+    assert torch.equal(w.grad, dw + db)
+    o.add_layer_norm(x, dy, w, w)[0].backward(dy)
+    dw2, db2 = torch.autograd.grad(o.add_layer_norm(x, dy, a, b)[0], (a, b), dy)
+    assert torch.equal(w.grad, (dw + db) + (dw2 + db2))       # the order of the additions: a pass's two, then into .grad
