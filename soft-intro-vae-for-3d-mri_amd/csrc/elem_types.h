@@ -34,15 +34,6 @@ __device__ __forceinline__ void store_stream(T* p, const Pack<T>& v) {
     __builtin_memcpy(&w, v.e, 16);
     __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
 }
-// An operand that nothing is expected to read again soon.
-template <typename T>
-__device__ __forceinline__ Pack<T> load_stream(const T* p) {
-    typedef uint32_t words __attribute__((ext_vector_type(4)));
-    const words w = __builtin_nontemporal_load(reinterpret_cast<const words*>(p));
-    Pack<T> v;
-    __builtin_memcpy(v.e, &w, 16);
-    return v;
-}
 // `have` elements of the row are left at p (<= 0: none, the pack is zero; >= N: a whole one).  AL: p is 16-byte
 // aligned and have is a multiple of N.  Otherwise p has the element's alignment only: the hardware takes a 16-byte
 // access at any address, so whole packs still are one instruction.
