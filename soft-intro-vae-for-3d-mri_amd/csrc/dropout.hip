@@ -8,6 +8,7 @@
 namespace siv {
 
 // What a call does beyond the product with the mask; OTHER is the residual (forward) or x (backward of an activation).
+// (ACT_RES: siv_dropout_fwd and the backend's dropout_fwd with a slope and a residual; siv.ops calls one or the other.)
 enum What { PLAIN, ACT, RES, ACT_RES, BWD_ACT };
 
 // A block takes a tile of 256 x P packs of 16 bytes, P to a thread, all requested before the first is worked on.  A tile

@@ -1,4 +1,5 @@
-"""Layer norm, dropout and the residual step called through what torch puts around an operator: a recorded trace."""
+"""Layer norm, dropout and the residual step called through what torch puts around an operator -- recorded traces, function
+transforms, hooks on saved tensors, one parameter twice -- and dropout behind an activation in every type."""
 import pytest
 import torch
 
@@ -190,3 +191,38 @@ def test_one_parameter_as_weight_and_bias(hip, R, C):
     o.add_layer_norm(x, dy, w, w)[0].backward(dy)
     dw2, db2 = torch.autograd.grad(o.add_layer_norm(x, dy, a, b)[0], (a, b), dy)
     assert torch.equal(w.grad, (dw + db) + (dw2 + db2))       # the order of the additions: a pass's two, then into .grad
+
+
+# ---- dropout behind an activation ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("slope", [0.0, 0.2, 1.0])
+@pytest.mark.parametrize("shape", [(1,), (5,), (13, 77), (70001,), (2, 3, 5, 7, 4)])
+def test_act_dropout_of_every_type(hip, shape, slope, dtype):
+    """LeakyReLU, dropout from a key, and (backend and C entry point) a residual: float64 values within a product's, a scaling's
+    and an addition's roundings in fp32 and one to the type; the gradient likewise."""
+    from siv import ops as o
+    u, half = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * half
+    fmt = CL3D if len(shape) == 5 else torch.contiguous_format
+    x, dy, res = (rnd(s, *shape, dtype=dtype).contiguous(memory_format=fmt) for s in (1, 2, 3))
+    k, p = key(2 ** 63 + 9, (3 << 40) | 17), 0.35
+    m = hip.dropout_keep(shape if len(shape) == 5 else (1, 1, 1, 1, x.numel()), x.device, p, k.seed, k.stream_id)
+    m = (m if len(shape) == 5 else m.view(shape)).double()
+    one = torch.tensor(1.0)
+    sc, a = float(one / (one - torch.tensor(p))), float(torch.tensor(slope))
+    xg = x.clone().requires_grad_()
+    out = o.act_dropout(xg, slope, k, p)
+    x64 = x.double()
+    ref = torch.where(x64 > 0, x64, a * x64) * m * sc
+    assert out.dtype == dtype and bool(((out.double() - ref).abs() <= (half + 2 * u) * ref.abs() + tiny).all())
+    dx, = torch.autograd.grad(out, xg, dy)
+    gref = dy.double() * m * sc * torch.where(x64 > 0, 1.0, a)
+    assert bool(((dx.double() - gref).abs() <= (half + 2 * u) * gref.abs() + tiny).all())
+    got = hip.dropout_fwd(x, k, p, slope, res)
+    both = res.double() + ref
+    assert bool(((got.double() - both).abs() <= (half + u) * both.abs() + 2 * u * ref.abs() + tiny).all())
+    assert torch.equal(got, hip.dropout_fwd(x, m.to(torch.uint8), p, slope, res))
+    raw = torch.empty_like(x)
+    rc = hip.lib.siv_dropout_fwd(x.data_ptr(), res.data_ptr(), None, k.seed, k.stream_id, None, p, slope, raw.data_ptr(),
+                                 hip._TYPES[dtype], x.numel(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(raw, got)
