@@ -185,3 +185,28 @@ def test_dropout_walks(hip, n, dtype):
     assert torch.equal(out, twice.clamp_min(0))
     dx, = torch.autograd.grad(out, xg, res.detach())
     assert torch.equal(dx, (2 * res.detach()).masked_fill_(~m | (x.detach() <= 0), 0))
+
+
+# ---- long rows beyond a grid's 65535 -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("C", [8200, 16392])
+def test_more_long_rows_than_a_grid_holds(hip, C):
+    """65541 chunked rows: the blocks of the statistics, of the forward pass (16392) and of the backward pass walk."""
+    if torch.cuda.mem_get_info()[0] < 200 << 30:
+        pytest.skip("needs 200 GB of device memory")
+    check_norm(65541, C, BF16)
+
+
+# ---- parameters at odd addresses ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("wdtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("C", [5, 64, 601, 1200, 9001])
+def test_parameters_at_odd_addresses(hip, C, wdtype):
+    from siv import ops as o
+    x, dy, w, b = B.inputs(7, C, BF16, C, "cuda")
+    w, b = w.to(wdtype), b.to(wdtype)
+    wide = torch.zeros(2 * C + 5, dtype=wdtype, device="cuda")
+    wide[1:1 + C], wide[C + 4:2 * C + 4] = w, b
+    x.requires_grad_()
+    got = [o.layer_norm(x, wide[1:1 + C], wide[C + 4:2 * C + 4])]
+    want = [o.layer_norm(x, w, b)]
+    assert torch.equal(got[0], want[0])
+    assert torch.equal(*(torch.autograd.grad(y[0], x, dy)[0] for y in (got, want)))
