@@ -88,15 +88,18 @@ static void dropout_launch(int what, const T* in, const T* other, const Drop& d,
 }
 // Packs per thread and grid.  fp32 is bound by HBM: one pack a thread and a block per tile (78.6 M elements: 107 us =
 // 5.9 TB/s; a grid of 4096 that walks the tensor 118, two packs 110).  Of 16-bit types a pack is two Philox calls, whose
-// arithmetic is as long as their traffic: several packs a thread, and for tensors that fill the chip many times over a
-// block per tile (315 M elements of bf16: 220-241 us with four packs, 256 with two, 258 with two and a grid of 2048), for
-// smaller ones a grid of 2048 (19.7 M: 14 us; block per tile 15.5 with two packs, 16.6 with four).  BIG lies between.
-constexpr long BLOCKS_MAX = 1L << 20, BIG = 1L << 27;
+// arithmetic is as long as their traffic: several packs a thread.  A call whose operands fit the Infinity Cache (256 MB)
+// runs two packs over a grid of 2048, a larger one a block per tile, with four packs where there is one operand.  Measured
+// on both sides in turn (us, bf16; grid of 2048 | block per tile): one operand 16.8 M elements 11.8 | 13.6, 50 M 32.5 | 34.3,
+// 67 M (268 MB) 42.6 | 43.7, 101 M 74.3 | 70.3, 315 M 245 | 226; onto a residual 33.6 M (201 MB) 35.1 | 34.6, 50 M (302 MB)
+// 62.9 | 54.8, 101 M 129 | 105, 315 M 410 | 323.
+constexpr long BLOCKS_MAX = 1L << 20, CACHE = 256L << 20;
 template <typename T, bool AL>
 static void dropout_size(int what, const T* in, const T* other, const Drop& d, float slope, T* out, long n,
                          hipStream_t st) {
+    const long bytes = n * (other ? 3 : 2) * (long)sizeof(T);
     if constexpr (sizeof(T) == 4) dropout_launch<T, 1, AL>(what, in, other, d, slope, out, n, BLOCKS_MAX, st);
-    else if (n >= BIG) dropout_launch<T, 4, AL>(what, in, other, d, slope, out, n, BLOCKS_MAX, st);
+    else if (bytes > CACHE) dropout_launch<T, 4, AL>(what, in, other, d, slope, out, n, BLOCKS_MAX, st);
     else dropout_launch<T, 2, AL>(what, in, other, d, slope, out, n, 2048, st);
 }
 static int dropout(const char* name, int what, const void* in, const void* other, const Drop& d, float slope, void* out,

@@ -159,7 +159,8 @@ def test_parameter_gradients_beyond_32_bit_offsets(hip):
 
 
 # ---- dropout: blocks that walk over the tensor ------------------------------------------------------------------------------
-@pytest.mark.parametrize("n,dtype", [(9_000_003, BF16), (9_000_003, F16), (20_000_001, BF16), ((1 << 27) + 4099, BF16),
+@pytest.mark.parametrize("n,dtype", [(9_000_003, BF16), (9_000_003, F16), (20_000_001, BF16), (44_739_243, F16),
+                                     (50_000_001, BF16), ((1 << 26) + 4099, F16), ((1 << 27) + 4099, BF16),
                                      ((1 << 30) + 5003, F32)])
 def test_dropout_walks(hip, n, dtype):
     """Two packs a thread over a grid of 2048, four and one over a grid of 2^20: every bit is the stored mask's, with and
