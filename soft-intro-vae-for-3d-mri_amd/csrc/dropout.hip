@@ -2,7 +2,7 @@
 // Element i of a call is component i % 4 of Philox(i / 4, stream id, seed): forward and backward draw it again instead
 // of writing and reading a mask.  Bytes: one tensor read and one written (two read onto a residual).  Arithmetic: per
 // four elements 18 products of 32 x 32 bits and 18 three-way xors; with 16-bit elements that takes about as long as
-// the traffic.  315 M elements of bf16: 220 us = 5.7 TB/s (a device copy: 237-285 us); 78.6 M of fp32: 108 us = 5.8.
+// the traffic.  315 M elements of bf16: 214-234 us = 5.4-5.9 TB/s (a device copy: 278 us); 78.6 M of fp32: 108 us = 5.8.
 #include "elem_types.h"
 
 namespace siv {

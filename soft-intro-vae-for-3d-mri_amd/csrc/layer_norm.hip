@@ -8,11 +8,12 @@
 //
 // Bound by HBM: forward reads and writes the tensor once, backward reads two and writes one (residual form: two and two,
 // three and two).  What the kernels move is that: WRITE_SIZE of a 4915200 x 64 fp32 call (1.26 GB tensors) is the tensor
-// to 0.04 %.  Times below: back-to-back calls on one MI355X, TB/s of those bytes; a device copy of that size runs at
-// 4.5-5.2.  4915200 x 64 fp32: forward 441 us (5.7), backward 664 us (5.7); residual form 614400 x 128 fp32: 227 (5.5) and
-// 304 us (5.2).  With 16-bit elements the arithmetic of the backward pass (about 16 operations an element on a lane that
-// holds eight) is close behind: 614400 x 128 bf16 forward 56 us (5.6), backward 88 us (5.4); 100000 x 601, where 52 of 128
-// lanes have no column, 111 us (3.2).
+// to 0.04 %.  Back-to-back calls of this build on one MI355X (profiles/norm_dropout_shapes.txt), TB/s of those bytes, where a
+// device copy of that size runs at 4.5-5.2: 4915200 x 64 fp32 forward 437 us (5.8), backward 667 us (5.7); residual form
+// 614400 x 128 fp32 228 (5.5) and 305 us (5.2).  With 16-bit elements the arithmetic of the backward pass (about 16
+// operations an element on a lane that holds eight) is close behind: 614400 x 128 bf16 forward 61 us (5.2), backward 92 us
+// (5.2); 100000 x 601, where 52 of 128 lanes have no column, 110 us (3.3).  Where a comment below gives two times for a
+// choice, they are of one series on the build of that day: the difference is meant, not the level.
 #include <algorithm>
 #include "elem_types.h"
 
@@ -345,7 +346,10 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_fwd_k(NormArgs a, 
 
 // The same rows backward.  Each lane sums dy h and dy of its columns over the rows it sees; a block's sums go to
 // a.part, or straight to the results where there is one block.  x and dy of the wave form, which nothing is expected to
-// read after this, are loaded non-temporally (4915200 x 64 fp32: 697 -> 668 us, 614400 x 128 bf16 104 -> 96).
+// read after this, are loaded non-temporally.  That pays where a call moves more than the Infinity Cache holds and costs where
+// it moves less (us, plain | non-temporal, profiles/norm_dropout_rules.txt): 4915200 x 64 fp32 706 | 684, 614400 x 128 bf16
+// 92.8 | 84.7, 153600 x 256 bf16 (236 MB) 48.5 | 45.6; 76800 x 256 bf16 (118 MB) 25.0 | 26.5, 200000 x 33 fp32 (79 MB)
+// 20.3 | 22.8.  One hint for all sizes: the large tensors are where the time is.
 template <typename T, int NV, int NT, int R, int COLS, bool RES>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT * R) void ln_bwd_k(NormArgs a, Drop d) {
     constexpr int N = Pack<T>::N;
@@ -766,11 +770,11 @@ __global__ __launch_bounds__(1024) void ln_param_sum_k(const float* __restrict__
 
 // ---- host -------------------------------------------------------------------------------------------------------------
 // The forms, by packs of 16 bytes in a row (fp32: 4 elements, 16-bit: 8).  Up to 64: lanes of one wave.  Up to 128: forward
-// two packs to a lane (100000 x 601 bf16: 56 us, 64 with a pack to each of 128 threads), backward 128 threads, since two
-// packs' sums and gradients need 168 registers.  Then a thread per pack up to 1024, four, two or one rows to a block so
-// that a block's partial sums stand for several rows (20000 x 1024 bf16 backward: one row to a block 39 us, four 28).
+// two packs to a lane (100000 x 601 bf16: 47 us; 56 against 64 with a pack to each of 128 threads), backward 128 threads,
+// since two packs' sums and gradients need 168 registers.  Then a thread per pack up to 1024, four, two or one rows to a block so
+// that a block's partial sums stand for several rows (20000 x 1024 bf16 backward: 25 us; one row to a block 39, four 28).
 // Up to 2048: two packs a thread, except 16-bit backward, which spills.  Longer rows: chunks, whose second read costs half as
-// much again (300 x 100000 fp32: forward 63 us = 5.7 TB/s of three passes, backward 112 us = 5.4 of five).
+// much again (300 x 100000 fp32: forward 59 us = 6.1 TB/s of three passes, backward 110 us = 5.5 of five).
 // Which kernel: a function of the row length and stride, the type and the direction alone, so that a row's result does
 // not depend on what is computed beside it.
 struct Form {

@@ -746,7 +746,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """nn.LayerNorm over the channels of every voxel (5-D tensors, NCDHW) or over the last axis (any other rank):
     ``(x - mean) / sqrt(var + eps) * weight + bias`` with the row's own mean and biased variance -- no batch, no running
     statistics.  float32, bfloat16 or float16; ``weight`` / ``bias`` float32 or of x's type, or None.  Rows may be slices
-    of wider rows.  Statistics are fp32 and formed again by the backward pass; only ``x`` is kept."""
+    of wider rows.  Statistics are fp32 and formed again by the backward pass; only ``x`` is kept.  First derivatives only
+    (as of ``dropout`` and ``add_layer_norm``); torch.func transforms, batched gradients and make_fx are refused."""
     nodes = _nodes()
     if nodes is not None:
         y = nodes.layer_norm(x, weight, bias, eps, _grad_buf(weight), _grad_buf(bias))

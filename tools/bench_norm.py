@@ -16,7 +16,8 @@ ROWS = [(4915200, 64, "fp32"), (614400, 128, "fp32"), (614400, 128, "bf16"), (76
         (20000, 1024, "bf16"), (16384, 2048, "fp32"), (8192, 4096, "fp32"), (8192, 8192, "bf16"), (2000, 16384, "bf16"),
         (300, 100000, "fp32"), (8, 38400, "fp16"), (100000, 601, "bf16"), (1050, 601, "bf16"), (200000, 33, "fp32"),
         (4, 600, "fp32")]
-FLAT = [(314572800, "bf16"), (78643200, "fp32"), (78643201, "fp32"), (19660800, "bf16"), (787101, "fp16"), (9600, "fp32")]
+FLAT = [(314572800, "bf16"), (78643200, "fp32"), (78643201, "fp32"), (19660800, "bf16"),
+        (50331648, "bf16"), (100663296, "bf16"), (787101, "fp16"), (9600, "fp32")]
 
 
 def timeit(fns, reps):
