@@ -788,13 +788,13 @@ class HipBackend:
     def _launch(self, what, x, *args):
         """Call the entry point ``what`` on the current stream of x's device, with that device current.  (The raw
         accessors: torch.cuda.current_stream / current_device cost microseconds on autograd's threads.)"""
-        dev = x.get_device()
         fn = getattr(self.lib, what)
-        if torch._C._cuda_getDevice() == dev:
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        # (the device is asked for where it is used: torch.compile with dynamic shapes makes a local number symbolic)
+        if torch._C._cuda_getDevice() == x.get_device():
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(x.get_device()))
         else:
-            with torch.cuda.device(dev):
-                rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            with torch.cuda.device(x.get_device()):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(x.get_device()))
         if rc != 0:
             _lib.check(rc, what)
 

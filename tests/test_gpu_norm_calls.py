@@ -226,3 +226,25 @@ def test_act_dropout_of_every_type(hip, shape, slope, dtype):
     rc = hip.lib.siv_dropout_fwd(x.data_ptr(), res.data_ptr(), None, k.seed, k.stream_id, None, p, slope, raw.data_ptr(),
                                  hip._TYPES[dtype], x.numel(), torch.cuda.current_stream().cuda_stream)
     assert rc == 0 and torch.equal(raw, got)
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+@pytest.mark.parametrize("i", [0, 2, 4, 5])
+def test_compiled_functions_compute(hip, i, dynamic):
+    """torch.compile runs the operators between its graphs, for fixed and for changing shapes, volumes in either order."""
+    from siv import ops as o
+    torch._dynamo.reset()
+    m = {n: (torch.rand(n, 6, 3, 4, 5, device="cuda") > 0.5).to(torch.uint8) for n in (2, 3)}
+
+    def f(x, r, w, b):
+        return masked_operators(o, m[x.shape[0]])[i](x * 2, r, w, b) + 1
+    run = torch.compile(f, backend="eager", dynamic=dynamic)
+    for n, fmt in ((2, CL3D), (3, CL3D), (3, torch.contiguous_format)):
+        args = [t.contiguous(memory_format=fmt).requires_grad_() for t in (rnd(n, n, 6, 3, 4, 5), rnd(n + 5, n, 6, 3, 4, 5))]
+        args += [rnd(3, 6).requires_grad_(), rnd(4, 6).requires_grad_()]
+        dy = rnd(9, n, 6, 3, 4, 5)
+        want, got = f(*args), run(*args)
+        assert torch.equal(got, want)
+        for a, c in zip(*(torch.autograd.grad(y, args, dy, allow_unused=True) for y in (got, want))):
+            assert a is c or torch.equal(a, c)
+    torch._dynamo.reset()
